@@ -32,8 +32,9 @@
 extern "C" {
 #endif
 
-/* Element types (torch.float32 / float16 / bfloat16 / int8 / int64). */
-enum b2k_dtype { B2K_F32 = 0, B2K_F16 = 1, B2K_BF16 = 2, B2K_I8 = 3, B2K_I64 = 4 };
+/* Element types (torch.float32 / float16 / bfloat16 / int8 / int64 /
+ * float8_e4m3fn). */
+enum b2k_dtype { B2K_F32 = 0, B2K_F16 = 1, B2K_BF16 = 2, B2K_I8 = 3, B2K_I64 = 4, B2K_E4M3 = 5 };
 
 enum b2k_status {
   B2K_OK = 0,
@@ -294,6 +295,94 @@ int b2k_entropy(const void* x, int64_t ldx, void* out, int64_t M, int64_t N,
  * Replaces kl_div (specs.py:860-864, reference :259-265). */
 int b2k_kl_div(const void* x, int64_t ldx, const void* y, int64_t ldy,
                void* out, int64_t M, int64_t N, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Low-precision serving operators (no reference counterparts). */
+
+/* [Residual addition] -> RMS norm -> *w -> 8 bits with fp32 scales:
+ *   h = T(x + r), y = (h*w) * rsqrt(mean(h^2) + eps) in fp32,
+ *   scale = max|y| / Q, q = round(y * Q / max|y|) over a row (group = 0) or
+ *   over every `group` (32, 64, 128) columns; Q = 127 for qtype B2K_I8, 448
+ *   for B2K_E4M3.  A maximum below 1e-30 gives scale 0 and q = 0; a NaN goes
+ *   into the scale.
+ *   r, h  : residual and residual-stream output (NULL = none; h needs r)
+ *   q     : (M,N) bytes with row stride ldq
+ *   scale : (M, group ? ceil(N/group) : 1) fp32 with row stride lds */
+int b2k_norm_quant(const void* x, int64_t ldx, const void* r, int64_t ldr, const void* w,
+                   void* h, int64_t ldh, void* q, int64_t ldq, float* scale, int64_t lds,
+                   int64_t M, int64_t N, int dtype, int qtype, int group, float eps,
+                   void* stream);
+
+/* The 4-bit paged key/value cache.  The pool `data` (16-byte aligned) is
+ * [pages, Hk, P/16] micro blocks of 16*(D + 8*D/group) bytes, one per 16
+ * tokens of one head: 16 key rows of D/2 bytes, 16 x D/group pairs (s, lo) of
+ * float16, 16 value rows, their pairs.  Value rows hold dimension i in nibble
+ * i, low bits first; key rows hold 32-bit words of eight dimensions, word
+ * c*(D/32) + j being dimensions 32j + 8c .. + 7.  A group of dimensions stands
+ * for lo + n*s, s = f16((max-min)/15), lo = f16(min),
+ * n = clamp(rint((x-lo)/s), 0, 15), inputs clamped to +-65408.
+ * D in {64, 128, 256}, group in {32, 64, 128} up to D, P a multiple of 16;
+ * slot = page*P + offset. */
+
+/* Quantises k, v (T tokens x Hk heads x D, 16-bit dtype, strides ld* between
+ * tokens and hd* between heads in elements) into the slots (distinct); slots
+ * outside [0, pages*P) are skipped. */
+int b2k_kv4_write(const void* k, int64_t ldk, int64_t hdk, const void* v, int64_t ldv,
+                  int64_t hdv, const int64_t* slots, int64_t T, void* data, int64_t pages,
+                  int64_t Hk, int64_t P, int64_t D, int64_t group, int dtype, void* stream);
+
+/* Reads slots back into contiguous k, v (T, Hk, D) of a 16-bit dtype: zeros
+ * for a negative slot, NaN for one past the pool. */
+int b2k_kv4_read(const void* data, int64_t pages, int64_t Hk, int64_t P, int64_t D,
+                 int64_t group, const int64_t* slots, int64_t T, void* k, void* v, int dtype,
+                 void* stream);
+
+/* Bytes of device workspace of b2k_kv4_attention at these sizes on the current
+ * device (the same for every length; -1 for invalid sizes). */
+int64_t b2k_kv4_attention_workspace(int64_t B, int64_t Sq, int64_t H, int64_t Hk, int64_t D);
+
+/* Attention of q (B, Sq, H, D; strides qb, qs, qh in elements) over the cached
+ * tokens of B sequences: table (B, width) holds each one's pages in order
+ * (entries past its length are not read), lens (B) its tokens, the Sq new ones
+ * included.  Head h reads cache head h / (H/Hk).  With causal != 0 query i
+ * sees tokens up to lens - Sq + i.  o (B, Sq, H, D) contiguous in dtype;
+ * lse (B, H, Sq) fp32 or NULL.  A row that sees nothing is zeros (lse -inf);
+ * a length beyond width*P, or a page outside the pool among the tokens read,
+ * gives NaN for the rows concerned.  The workspace is scratch of
+ * b2k_kv4_attention_workspace bytes (16-byte aligned), needs no
+ * initialisation, and is free again when the call's GPU work has run. */
+int b2k_kv4_attention(const void* q, int64_t qb, int64_t qs, int64_t qh, void* o, float* lse,
+                      const void* data, int64_t pages, int64_t Hk, int64_t P, int64_t D,
+                      int64_t group, const int32_t* table, int64_t width, const int32_t* lens,
+                      int64_t B, int64_t Sq, int64_t H, float scale, int causal, int dtype,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
+/* 4-bit weights W[n,k] = s[n,k/group] * (w[n,k] - z[n,k/group]), w in 0..15,
+ * z = 8 without zeros, group 32 / 64 / 128, s and z of a 16-bit stype.
+ * Laid out as tiles [ceil(N/16), ceil(K/128), 16 rows, 64 bytes], 32-bit word
+ * 4c + j of a row holding columns 32j + 8c .. + 7 of its 128 (the first column
+ * in the low bits), and scales / zeros [ceil(N/16), ceil(K/128), 128/group,
+ * 16]; what lies past N or K is 0. */
+
+/* Lays out integers q (N,K) and scales / zeros (N, ceil(K/group)). */
+int b2k_w4_pack(const uint8_t* q, int64_t ldq, const void* scales, const void* zeros,
+                int64_t lds, int64_t N, int64_t K, int group, int stype, void* tiles,
+                void* tile_scales, void* tile_zeros, void* stream);
+
+/* Rounds weights w (N,K) of a floating dtype to that form: s = max|w| / 7
+ * without zeros (tile_zeros NULL), else (max - min) / 15 over the group's
+ * values and 0, with z the whole number that stands for 0. */
+int b2k_w4_quantize(const void* w, int64_t ldw, int64_t N, int64_t K, int dtype, int group,
+                    int stype, void* tiles, void* tile_scales, void* tile_zeros, void* stream);
+
+/* y (M,N) = x (M,K) W^T with fp32 sums.  x is a floating dtype, or B2K_I8 /
+ * B2K_E4M3 with fp32 scales xs (M, xgroup ? ceil(K/xgroup) : 1), xgroup a
+ * multiple of the weight's group up to 128.  y is a floating dtype.  A row of
+ * x that holds an infinity or a NaN gives NaN. */
+int b2k_w4_matmul(const void* x, int64_t ldx, int xtype, const float* xs, int64_t ldxs,
+                  int xgroup, const void* tiles, const void* tile_scales,
+                  const void* tile_zeros, int stype, int group, int64_t M, int64_t N,
+                  int64_t K, void* y, int64_t ldy, int ytype, void* stream);
 
 #ifdef __cplusplus
 }

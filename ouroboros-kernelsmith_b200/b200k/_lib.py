@@ -14,7 +14,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libb200k.so")
 
 # enum values mirrored from include/b200k.h
-F32, F16, BF16, I8, I64 = 0, 1, 2, 3, 4
+F32, F16, BF16, I8, I64, E4M3 = 0, 1, 2, 3, 4, 5
 OK, EINVAL, EALIGN, ELAUNCH, EUNSUPPORTED = 0, 1, 2, 3, 4
 NORM_RMS, NORM_L2, NORM_LN = 0, 1, 2
 AFF_NONE, AFF_W_ROUNDED, AFF_W, AFF_ONE_PLUS_W, AFF_WB = 0, 1, 2, 3, 4
@@ -76,6 +76,26 @@ SIGNATURES = {
     "b2k_entropy": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p]),
     "b2k_kl_div": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int,
                            c_void_p]),
+    "b2k_norm_quant": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
+                               c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int,
+                               c_int, c_int, c_float, c_void_p]),
+    "b2k_kv4_write": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
+                              c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64,
+                              c_int, c_void_p]),
+    "b2k_kv4_read": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                             c_int64, c_void_p, c_void_p, c_int, c_void_p]),
+    "b2k_kv4_attention_workspace": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64]),
+    "b2k_kv4_attention": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                                  c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                  c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_float,
+                                  c_int, c_int, c_void_p, c_int64, c_void_p]),
+    "b2k_w4_pack": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64,
+                            c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "b2k_w4_quantize": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_int,
+                                c_void_p, c_void_p, c_void_p, c_void_p]),
+    "b2k_w4_matmul": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p,
+                              c_void_p, c_void_p, c_int, c_int, c_int64, c_int64, c_int64,
+                              c_void_p, c_int64, c_int, c_void_p]),
 }
 
 

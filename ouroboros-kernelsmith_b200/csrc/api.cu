@@ -56,6 +56,7 @@ int dtype_size(int dtype) {
     case B2K_BF16: return 2;
     case B2K_I8: return 1;
     case B2K_I64: return 8;
+    case B2K_E4M3: return 1;
     default: return 0;
   }
 }
