@@ -63,6 +63,7 @@ def test_attention_refusals():
     refused(attention(dtype=L.F32), "dtype")
     refused(attention(q=None), "null")
     refused(attention(table=None), "null")
+    refused(attention(), "workspace")
     refused(attention(B=1 << 20, Sq=1 << 20), "too many")
     assert attention(B=0) == L.OK
     assert L.lib.b2k_kv4_attention_workspace(-1, 1, 8, 8, 128) == -1
