@@ -378,11 +378,15 @@ int b2k_w4_quantize(const void* w, int64_t ldw, int64_t N, int64_t K, int dtype,
 /* y (M,N) = x (M,K) W^T with fp32 sums.  x is a floating dtype, or B2K_I8 /
  * B2K_E4M3 with fp32 scales xs (M, xgroup ? ceil(K/xgroup) : 1), xgroup a
  * multiple of the weight's group up to 128.  y is a floating dtype.  A row of
- * x that holds an infinity or a NaN gives NaN. */
+ * x that holds an infinity or a NaN gives NaN.  Few rows of x are held on chip
+ * whole; where they do not fit, K is split and the workspace holds partial
+ * sums (b2k_w4_matmul_workspace bytes, 0 mostly; needs no initialisation). */
+int64_t b2k_w4_matmul_workspace(int64_t M, int64_t N, int64_t K, int group, int xtype);
 int b2k_w4_matmul(const void* x, int64_t ldx, int xtype, const float* xs, int64_t ldxs,
                   int xgroup, const void* tiles, const void* tile_scales,
                   const void* tile_zeros, int stype, int group, int64_t M, int64_t N,
-                  int64_t K, void* y, int64_t ldy, int ytype, void* stream);
+                  int64_t K, void* y, int64_t ldy, int ytype, void* workspace,
+                  int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -95,7 +95,8 @@ SIGNATURES = {
                                 c_void_p, c_void_p, c_void_p, c_void_p]),
     "b2k_w4_matmul": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p,
                               c_void_p, c_void_p, c_int, c_int, c_int64, c_int64, c_int64,
-                              c_void_p, c_int64, c_int, c_void_p]),
+                              c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p]),
+    "b2k_w4_matmul_workspace": (c_int64, [c_int64, c_int64, c_int64, c_int, c_int]),
 }
 
 

@@ -390,7 +390,9 @@ def w4_matmul(x, weight: W4Weight, *, x_scale=None, out_dtype: torch.dtype | Non
     y = torch.empty((m, n), dtype=out_dtype, device=dev)
     tiles, scales, zeros, st, _ = weight._args
     with _dev(dev) as stream:
+        nws = L.lib.b2k_w4_matmul_workspace(m, n, k, group, xt)
+        ws = torch.empty((nws,), dtype=torch.uint8, device=dev) if nws > 0 else None
         L.check(L.lib.b2k_w4_matmul(_p(x2), ldx, xt, _p(xs), ldxs, xg, tiles, scales, zeros, st,
-                                    group, m, n, k, _p(y), n, _DT[out_dtype], stream),
+                                    group, m, n, k, _p(y), n, _DT[out_dtype], _p(ws), nws, stream),
                 "b2k_w4_matmul")
     return y if x.dim() == 2 else y.view(x.shape[:-1] + (n,))

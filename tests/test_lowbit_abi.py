@@ -72,7 +72,7 @@ def test_attention_refusals():
 def product(N=64, K=128, M=2, xt=L.BF16, xs=None, xg=0, group=32, yt=L.BF16, y=FAKE, stype=L.F16,
             ldx=128):
     return L.lib.b2k_w4_matmul(FAKE, ldx, xt, xs, 4, xg, FAKE, FAKE, None, stype, group, M, N, K, y,
-                               64, yt, None)
+                               64, yt, None, 0, None)
 
 
 def test_product_refusals():
