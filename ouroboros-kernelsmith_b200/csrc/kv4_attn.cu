@@ -24,16 +24,18 @@
 //     meets probabilities in float16 (2^-11), sums in fp32.  Probabilities are
 //     held times 2^10, which keeps small ones out of the subnormals.
 //   * The running maximum and sum are fp32, per lane for its own tokens; the
-//     output is rescaled only when a maximum moves.
+//     output is rescaled only when a row's maximum has moved by 2^4.
 //
 // Work is split by tiles of tokens, not by sequences: all (sequence, row
-// tile, head) segments are laid end to end and every block takes an equal
-// run of tiles, found on the device from the lengths (which the host does not
-// know), so ragged batches and single long sequences fill the GPU alike.  A
-// segment that spans blocks leaves partial (m, l, O) in the workspace, merged
-// in block order by a second kernel (the same bits whatever ran first).
-// Within a block the warps take tiles in turn, each with its own ring of bulk
-// copies; they meet once per segment.
+// tile, head) segments are laid end to end and every warp takes an equal run
+// of tiles (a segment counts kAttnLead more for its own costs), found on the
+// device from the lengths, which the host does not know; so ragged batches and
+// single long sequences fill the GPU alike.  Warps are independent: each has
+// its own ring of bulk copies, which runs ahead across segments, and writes
+// the segments that it holds whole.  A segment that spans warps leaves partial
+// (m, l, O) in the workspace, merged in order by a second kernel (the same
+// bits whatever ran first); where all of a block's runs lie in one segment,
+// the long sequences, the block's warps merge theirs first.
 #include "kv4.cuh"
 #include "rowio.cuh"
 #include "tma.cuh"
@@ -48,9 +50,36 @@ int kv4_check(const char* what, const void* data, int64_t pages, int64_t Hk, int
 constexpr int kAttnWarps = 4;
 constexpr int kAttnStages = 3;
 constexpr float kPScale = 10.0f;  // probabilities are held times 2^10
+constexpr float kPSlack = 4.0f;   // ... and below 2^(10 + 4) until the maximum is moved
+constexpr int kAttnLead = 2;      // a segment's fixed costs, in tiles
+constexpr int kAttnLeast = 2;     // tiles of a run beside them
+
+// n / d for 0 <= n < 2^31 by a multiplication (d is known on the host):
+// with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1,
+// floor(n / d) = (hi32(m n) + n) >> s.
+struct FastDiv {
+  uint32_t d, m, s;
+  __device__ __forceinline__ int div(int n) const {
+    return (int)((__umulhi((uint32_t)n, m) + (uint32_t)n) >> s);
+  }
+};
+static FastDiv fast_div(int64_t d) {
+  FastDiv f;
+  f.d = (uint32_t)d;
+  f.s = 0;
+  while ((1ll << f.s) < d) ++f.s;
+  f.m = (uint32_t)(((1ull << 32) * ((1ull << f.s) - (uint64_t)d)) / (uint64_t)d + 1);
+  return f;
+}
+// 64-bit division that takes the short way for what fits 32 bits
+__device__ __forceinline__ int64_t wide_div(int64_t n, int64_t d) {
+  if (((n | d) >> 32) == 0) return (uint32_t)n / (uint32_t)d;
+  return n / d;
+}
 
 struct Kv4AttnArgs {
   Kv4 c;
+  FastDiv dG, dRT, dP, dHk;
   const void* q;
   void* o;
   float* lse;
@@ -59,9 +88,10 @@ struct Kv4AttnArgs {
   int64_t qb, qs, qh;  // strides of q in elements (batch, token, head)
   float scale;
   int causal, bf16, q_aligned;
+  int warps;  // of the launch
   int G, RT;  // query heads per cache head; row tiles per (sequence, head)
-  float* part;      // [2 * blocks][rows][D] outputs, then [2 * blocks][rows][2] (m, l)
-  int2* spans;      // [segments] first and last block
+  float* part;      // [2 * warps][rows][D] outputs, then [2 * warps][rows][2] (m, l)
+  int2* spans;      // [segments] first and last warp
 };
 
 // tokens of a tile: about the same bytes for every D, and registers for its
@@ -81,13 +111,13 @@ __device__ __forceinline__ int attn_len(const Kv4AttnArgs& a, int b, bool& bad) 
 // first token that no row of the row tile sees
 template <int D, int NT>
 __device__ __forceinline__ int attn_end(const Kv4AttnArgs& a, int len, int rt) {
-  const int last_row = (int)min((int64_t)(rt + 1) * attn_rows(NT), a.Sq * a.G) - 1;
-  return max(a.causal ? len - (int)a.Sq + last_row / a.G + 1 : len, 0);
+  const int last_row = min((rt + 1) * attn_rows(NT), (int)a.Sq * a.G) - 1;
+  return max(a.causal ? len - (int)a.Sq + a.dG.div(last_row) + 1 : len, 0);
 }
 // tiles of each of its segments (one at least: somebody writes the zeros)
 template <int D, int NT> __device__ __forceinline__ int attn_tiles(const Kv4AttnArgs& a, int entry) {
   bool bad;
-  const int b = entry / a.RT, end = attn_end<D, NT>(a, attn_len(a, b, bad), entry - b * a.RT);
+  const int b = a.dRT.div(entry), end = attn_end<D, NT>(a, attn_len(a, b, bad), entry - b * a.RT);
   return max((end + attn_tile(D, NT) - 1) / attn_tile(D, NT), 1);
 }
 
@@ -98,6 +128,15 @@ __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uin
       "{%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the same on zero sums
+__device__ __forceinline__ void mma16816_first(float* c, uint32_t a0, uint32_t a1, uint32_t a2,
+                                               uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
@@ -143,13 +182,70 @@ template <int D, int GRP, int NT> struct AttnShape {
   static constexpr int MB = 16 * (D + 8 * NG);           // bytes of a micro block
   static constexpr int KP = 8 * D, VR = KP + 64 * NG, VP = VR + 8 * D;  // its fields
   static constexpr int STAGE = U * MB;
-  static constexpr int RING = kAttnWarps * kAttnStages * STAGE;
   static constexpr int MERGE = kAttnWarps * ROWS * D * 4;
   // query fragments, and the groups' sums, in shared memory instead of registers
   static constexpr bool QS = NT * D > 128, GS = NT * NG > 4;
-  static constexpr int QB = (QS ? NT * J * 512 : 0) + (GS ? NT * NG * 32 : 0);
-  static constexpr int SMEM = (RING > MERGE ? RING : MERGE) + QB;
+  static constexpr int QB = QS ? NT * J * 512 : 0;
+  static constexpr int WARP = kAttnStages * STAGE + QB + (GS ? NT * NG * 32 : 0);
+  static constexpr int SMEM = kAttnWarps * WARP > MERGE ? kAttnWarps * WARP : MERGE;
 };
+
+// Four output values of 16 bits
+__device__ __forceinline__ uint2 attn_pack4(const float4& v, float f, int bf16) {
+  if (bf16) {
+    const __nv_bfloat162 p0 = __floats2bfloat162_rn(v.x * f, v.y * f);
+    const __nv_bfloat162 p1 = __floats2bfloat162_rn(v.z * f, v.w * f);
+    return make_uint2(*reinterpret_cast<const uint32_t*>(&p0), *reinterpret_cast<const uint32_t*>(&p1));
+  }
+  return make_uint2(as_u32(__floats2half2_rn(v.x * f, v.y * f)),
+                    as_u32(__floats2half2_rn(v.z * f, v.w * f)));
+}
+// 0 for a row that sees nothing; a NaN stays one
+__device__ __forceinline__ float attn_inverse(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+__device__ __forceinline__ float attn_lse(float m, float l) {
+  return l == 0.0f ? -INFINITY : (m - kPScale) * kLn2 + logf(l);
+}
+// factor of a part with maximum m and sum l in a merge to the maximum M; a
+// part that saw nothing counts 0, one made NaN before it saw anything NaN
+__device__ __forceinline__ float attn_weight(float m, float l, float M) {
+  return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : ex2_approx(m - M);
+}
+
+// (m, l) of a row of a partial slot, after the outputs of all slots
+__device__ __forceinline__ float2* attn_ml(const Kv4AttnArgs& a, int64_t slot_row, int slot_floats) {
+  return reinterpret_cast<float2*>(a.part + (int64_t)2 * a.warps * slot_floats) + slot_row;
+}
+
+// A walk over the parts of segments in a warp's run: tiles [t, t1) of segment
+// (entry, head), which has n.
+struct AttnWalk {
+  int entry, head, n, pos, left;  // pos: units of the segment already taken
+  int t, t1;
+};
+// on to the next part that has tiles
+template <int D, int NT> __device__ __forceinline__ bool attn_next(const Kv4AttnArgs& a, AttnWalk& k) {
+  while (k.left > 0) {
+    if (k.n == 0) k.n = attn_tiles<D, NT>(a, k.entry);
+    const int take = min(k.left, k.n + kAttnLead - k.pos);
+    k.t = max(k.pos - kAttnLead, 0);
+    k.t1 = max(k.pos + take - kAttnLead, 0);
+    k.left -= take;
+    k.pos += take;
+    if (k.t1 > k.t) return true;
+    // only the lead of a segment that goes on in the next warp's run
+  }
+  return false;
+}
+// past a finished part
+__device__ __forceinline__ void attn_step(const Kv4AttnArgs& a, AttnWalk& k) {
+  if (k.pos < k.n + kAttnLead) return;  // the run ends within the segment
+  k.pos = 0;
+  if (++k.head == a.c.Hk) {
+    k.head = 0;
+    k.n = 0;
+    ++k.entry;
+  }
+}
 
 template <int D, int GRP, int NT>
 __global__ void __launch_bounds__(32 * kAttnWarps, attn_cps(D, NT))
@@ -159,110 +255,159 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
   constexpr int VW = D / 64;  // words of a lane's D / 8 value dimensions
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint64_t full[kAttnWarps][S];
-  __shared__ int64_t scan[kAttnWarps + 1];
-  __shared__ int start_entry;
-  __shared__ int64_t start_rest;
+  __shared__ int ends[kAttnWarps], first_segment[2];
   __shared__ float mrg[kAttnWarps][X::ROWS][2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
-  unsigned char* ring = smem + warp * (S * X::STAGE);
-  uint32_t* qsm = reinterpret_cast<uint32_t*>(smem + X::SMEM - X::QB);
-  float* gsm = reinterpret_cast<float*>(smem + X::SMEM - (X::GS ? NT * NG * 32 : 0));
+  unsigned char* ring = smem + warp * X::WARP;
+  uint32_t* qsm = reinterpret_cast<uint32_t*>(ring + S * X::STAGE);
+  float* gsm = reinterpret_cast<float*>(ring + S * X::STAGE + X::QB);
 
   griddep_launch_dependents();
   if (lane < S) mbar_init(&full[warp][lane], 1);
   fence_barrier_init();
   griddep_wait();
 
-  // ---- this block's run of tiles -----------------------------------------
+  // ---- this warp's run: each lane sums the segments of some entries ----------
   const int entries = (int)(a.B * a.RT);  // (sequence, row tile), Hk segments each
-  const int chunk = (entries + (int)blockDim.x - 1) / (int)blockDim.x;
-  const int e0 = min(entries, tid * chunk), e1 = min(entries, e0 + chunk);
+  const int chunk = (entries + 31) / 32;
+  const int e0 = min(entries, lane * chunk), e1 = min(entries, e0 + chunk);
   int64_t mine = 0;
-  for (int e = e0; e < e1; ++e) mine += attn_tiles<D, NT>(a, e);
-  int64_t incl = mine;
+  for (int e = e0; e < e1; ++e) mine += attn_tiles<D, NT>(a, e) + kAttnLead;
+  int64_t before = mine;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t t = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += t;
+  for (int x = 1; x < 32; x <<= 1) {
+    const int64_t t = __shfl_up_sync(0xffffffffu, before, x);
+    if (lane >= x) before += t;
   }
-  if (lane == 31) scan[warp] = incl;
-  __syncthreads();
-  int64_t before = incl - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < kAttnWarps; ++w) {
-    if (w < warp) before += scan[w];
-    total += scan[w];
+  const int64_t total = __shfl_sync(0xffffffffu, before, 31) * a.c.Hk;
+  mine *= a.c.Hk;
+  before = before * a.c.Hk - mine;
+  // a run is a segment's lead and kAttnLeast tiles at least; the first `more`
+  // runs are one unit longer than `each`
+  const int64_t runs = min((int64_t)gridDim.x * kAttnWarps,
+                           wide_div(total + kAttnLead + kAttnLeast - 1, kAttnLead + kAttnLeast));
+  const int64_t each = wide_div(total, runs), more = total - each * runs;
+  auto run_at = [&](int64_t i) { return i * each + min(i, more); };
+  auto run_of = [&](int64_t u) {
+    return u < more * (each + 1) ? wide_div(u, each + 1) : more + wide_div(u - more * (each + 1), each);
+  };
+  const int64_t run0 = (int64_t)blockIdx.x * kAttnWarps, run = run0 + warp;
+  if (run0 >= runs) return;
+  AttnWalk use = {};
+  bool one_segment = false;  // of all the block's runs
+  const int64_t u1 = run_at(min(run + 1, runs));
+  if (run < runs) {
+    const int64_t u0 = run_at(run);
+    int64_t at = u0 - before;
+    const bool here = at >= 0 && at < mine;
+    int e = e0, n = 0;
+    if (here)
+      for (;; ++e) {
+        n = attn_tiles<D, NT>(a, e);
+        const int64_t all = (int64_t)(n + kAttnLead) * a.c.Hk;
+        if (at < all) break;
+        at -= all;
+      }
+    const int src = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+    use.entry = __shfl_sync(0xffffffffu, e, src);
+    use.n = __shfl_sync(0xffffffffu, n, src);
+    at = __shfl_sync(0xffffffffu, at, src);
+    use.head = (int)wide_div(at, use.n + kAttnLead);
+    use.pos = (int)(at - (int64_t)use.head * (use.n + kAttnLead));
+    use.left = (int)(u1 - u0);
+    const int64_t base = u0 - use.pos;  // of the segment
+    one_segment = base <= run_at(run0) &&
+                  run_at(min(run0 + kAttnWarps, runs)) <= base + use.n + kAttnLead;
   }
-  before *= a.c.Hk;
-  total *= a.c.Hk;
-  // a block has at least one tile per warp
-  const int64_t blocks = min((int64_t)gridDim.x, (total + kAttnWarps - 1) / kAttnWarps);
-  const int64_t me = blockIdx.x;
-  if (me >= blocks) return;
-  const int64_t u0 = me * total / blocks, u1 = (me + 1) * total / blocks;
-  if (u0 >= before && u0 < before + mine * a.c.Hk) {
-    int64_t at = before;
-    int e = e0;
-    for (;; ++e) {
-      const int64_t n = (int64_t)attn_tiles<D, NT>(a, e) * a.c.Hk;
-      if (u0 < at + n) break;
-      at += n;
-    }
-    start_entry = e;
-    start_rest = u0 - at;
-  }
-  __syncthreads();
-
-  int entry = start_entry;
-  int64_t unit = u0;
-  int n_seg = attn_tiles<D, NT>(a, entry);
-  int head = (int)(start_rest / n_seg);
-  int t0 = (int)(start_rest - (int64_t)head * n_seg);  // first tile of this part
-  uint32_t issued = 0, used = 0;                       // stages, over the whole block
+  // the warps past the last run join the merge of the others
+  one_segment = __syncthreads_or(one_segment) != 0;
+  AttnWalk get = use;
+  uint32_t issued = 0, used = 0;  // stages
   bool timeout = false;
 
-  while (unit < u1 && !timeout) {
-    const int b = entry / a.RT, rt = entry - b * a.RT;
-    bool bad;
+  // ---- the ring: the walk `get` runs ahead of `use` by up to S tiles ---------
+  // lane l < U fetches the 16 tokens from `get_tok` of its page, which it looked
+  // up one tile before
+  int get_tok = 0, get_off = 0, get_end = 0, get_pid = 0;
+  const int32_t* get_page = nullptr;
+  bool getting = false, bad = false, my_first = false, my_last = false;
+  uint32_t bad_stages = 0;  // a page outside the pool among the tokens of a stage
+  const int64_t head_bytes = (int64_t)(a.c.P >> 4) * MB;
+  auto open = [&]() {  // the next part's first tile
+    getting = attn_next<D, NT>(a, get);
+    if (getting) {
+      const int b = a.dRT.div(get.entry);
+      bool over;
+      get_end = lane < U ? attn_end<D, NT>(a, attn_len(a, b, over), get.entry - b * a.RT) : 0;
+      get_tok = get.t * T + (lane < U ? 16 * lane : 0);
+      const int pi = a.dP.div(get_tok);
+      get_page = a.table + b * a.width + pi;
+      get_off = get_tok - pi * a.c.P;
+      get_pid = get_tok < get_end ? *get_page : -1;
+    }
+  };
+  auto issue = [&]() {
+    const int s = issued % S;
+    const bool have = get_tok < get_end && get_pid >= 0 && get_pid < a.c.pages;
+    const uint32_t got = __ballot_sync(0xffffffffu, have);
+    const uint32_t miss = __any_sync(0xffffffffu, get_tok < get_end && !have) ? 1u : 0u;
+    bad_stages = (bad_stages & ~(1u << s)) | (miss << s);
+    fence_proxy_async();
+    if (lane == 0) mbar_arrive_expect_tx(&full[warp][s], __popc(got) * MB);
+    __syncwarp();
+    if (have)
+      bulk_g2s(ring + s * X::STAGE + lane * MB,
+               a.c.data + ((int64_t)get_pid * a.c.Hk + get.head) * head_bytes + (get_off >> 4) * MB, MB,
+               &full[warp][s]);
+    ++issued;
+    if (++get.t == get.t1) {
+      attn_step(a, get);
+      open();
+    } else {
+      get_tok += T;
+      get_off += T;
+      while (get_off >= a.c.P) {
+        get_off -= a.c.P;
+        ++get_page;
+      }
+      get_pid = get_tok < get_end ? *get_page : -1;
+    }
+  };
+  open();
+  for (int k = 0; k < S && getting; ++k) issue();
+
+  float o[D / 16][NT][4];
+  float m[NT][2], l[NT][2];
+  auto clear = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.0f;
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.0f;
+    }
+  };
+  clear();
+
+  while (!timeout && attn_next<D, NT>(a, use)) {
+    const int b = a.dRT.div(use.entry), rt = use.entry - b * a.RT, head = use.head;
+    const int t0 = use.t, t1 = use.t1;
     const int len = attn_len(a, b, bad);
     const int end = attn_end<D, NT>(a, len, rt);
-    const int t1 = (int)min((int64_t)n_seg, t0 + (u1 - unit));  // one past its last tile
     const int R = (int)(a.Sq * a.G);
     const int row0 = rt * X::ROWS;
     // last token that a row of the tile sees
     auto last_of = [&](int row) {
-      return a.causal ? len - (int)a.Sq + min(row0 + row, R - 1) / a.G : len - 1;
+      return a.causal ? len - (int)a.Sq + a.dG.div(min(row0 + row, R - 1)) : len - 1;
     };
-
-    // ---- the ring: tile t of this warp into stage `issued` ----------------
-    const int32_t* pages = a.table + b * a.width;
-    auto issue = [&](int t) {
-      const int s = issued % S;
-      const int tok = t * T + (lane < U ? 16 * lane : 0);
-      bool have = false;
-      int page = 0;
-      if (lane < U && tok < end) {
-        page = pages[tok / a.c.P];
-        have = page >= 0 && page < a.c.pages;
-        if (!have) bad = true;
-      }
-      const uint32_t n = __popc(__ballot_sync(0xffffffffu, have));
-      fence_proxy_async();
-      if (lane == 0) mbar_arrive_expect_tx(&full[warp][s], n * MB);
-      __syncwarp();
-      if (have)
-        bulk_g2s(ring + s * X::STAGE + lane * MB, a.c.micro(page, head, tok % a.c.P), MB,
-                 &full[warp][s]);
-      ++issued;
-    };
-    int next = t0 + warp;  // tile of the next issue
-    for (int k = 0; k < S && next < t1; ++k, next += kAttnWarps) issue(next);
 
     // ---- query rows -> B fragments -----------------------------------------
     // lane (r, c) holds row r of each 8, dimensions 32 j + 8 c .. + 7
     uint32_t qf[X::QS ? 1 : NT][X::QS ? 1 : J][4];
     float qsum[X::GS ? 1 : NT][X::GS ? 1 : NG][2], cmul[NT][2];
-    if (X::QS || X::GS) __syncthreads();
+    if (X::QS || X::GS) __syncwarp();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int row = row0 + nt * 8 + r;
@@ -272,7 +417,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[j][e] = 0.0f;
       if (row < R) {
-        const int i = row / a.G, hq = head * a.G + (row - i * a.G);
+        const int i = a.dG.div(row), hq = head * a.G + (row - i * a.G);
         const int64_t off = b * a.qb + i * a.qs + hq * a.qh;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
@@ -312,9 +457,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
         uint32_t w[4] = {as_u32(__halves2half2(h[0], h[4])), as_u32(__halves2half2(h[2], h[6])),
                          as_u32(__halves2half2(h[1], h[5])), as_u32(__halves2half2(h[3], h[7]))};
         if constexpr (X::QS) {
-          if ((nt * J + j) % kAttnWarps == warp)
-            reinterpret_cast<uint4*>(qsm)[(nt * J + j) * 32 + lane] =
-                make_uint4(w[0], w[1], w[2], w[3]);
+          reinterpret_cast<uint4*>(qsm)[(nt * J + j) * 32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e) qf[nt][j][e] = w[e];
@@ -333,35 +476,26 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
         t += __shfl_xor_sync(0xffffffffu, t, 2);
         t *= 5.9604644775390625e-8f;  // 2^-24, the unit of the integers' products
         if constexpr (X::GS) {
-          if (nt % kAttnWarps == warp && c == 0) gsm[(nt * NG + g) * 8 + r] = t;
+          if (c == 0) gsm[(nt * NG + g) * 8 + r] = t;
         } else {
           qsum[nt][g][0] = __shfl_sync(0xffffffffu, t, 8 * c);
           qsum[nt][g][1] = __shfl_sync(0xffffffffu, t, 8 * c + 4);
         }
       }
     }
-    if (X::QS || X::GS) __syncthreads();
+    if (X::QS || X::GS) __syncwarp();
     const int all_see = last_of(0);  // tokens up to here are seen by every row
 
-    float o[D / 16][NT][4];
-    float m[NT][2], l[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.0f;
-      m[nt][0] = m[nt][1] = -INFINITY;
-      l[nt][0] = l[nt][1] = 0.0f;
-    }
+    clear();
 
-    for (int t = t0 + warp; t < t1; t += kAttnWarps) {
+    for (int t = t0; t < t1; ++t) {
       const int s = used % S;
       if (!mbar_wait(&full[warp][s], (used / S) & 1)) {
         timeout = true;
         break;
       }
       ++used;
+      bad |= (bad_stages >> s) & 1;
       unsigned char* st = ring + s * X::STAGE;
       const int tok0 = t * T;
       const bool masked = tok0 + T - 1 > all_see;
@@ -398,54 +532,61 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
 
       // ---- scores: [tokens] x [rows] ---------------------------------------
       float z[U][NT][4];
+      uint32_t kw[U][2][J], kp[U][2][NG];  // rows r and r + 8
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const unsigned char* mb = st + u * MB;
-        uint32_t wa[J], wb[J], pa[NG], pb[NG];
-        load_words<D / 8>(wa, mb + r * (D / 2) + c * (D / 8));
-        load_words<D / 8>(wb, mb + (r + 8) * (D / 2) + c * (D / 8));
-        load_words<4 * NG>(pa, mb + X::KP + r * 4 * NG);
-        load_words<4 * NG>(pb, mb + X::KP + (r + 8) * 4 * NG);
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int h = 0; h < 2; ++h) {
+          const unsigned char* mb = st + u * MB;
+          load_words<D / 8>(kw[u][h], mb + (r + 8 * h) * (D / 2) + c * (D / 8));
+          load_words<4 * NG>(kp[u][h], mb + X::KP + (r + 8 * h) * 4 * NG);
+        }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) z[u][nt][e] = 0.0f;
+      for (int g = 0; g < NG; ++g) {
+        float acc[U][NT][4];
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          float acc[NT][4];
+        for (int j = g * (GRP / 32); j < (g + 1) * (GRP / 32); ++j) {
+          uint32_t qv[NT][4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt) {
+            if constexpr (X::QS) {
+              const uint4 v = reinterpret_cast<const uint4*>(qsm)[(nt * J + j) * 32 + lane];
+              qv[nt][0] = v.x; qv[nt][1] = v.y; qv[nt][2] = v.z; qv[nt][3] = v.w;
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[nt][e] = 0.0f;
-#pragma unroll
-          for (int j = g * (GRP / 32); j < (g + 1) * (GRP / 32); ++j) {
-            const uint32_t ya = wa[j] >> 8, yb = wb[j] >> 8;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              uint32_t q4[4];
-              if constexpr (X::QS) {
-                const uint4 v = reinterpret_cast<const uint4*>(qsm)[(nt * J + j) * 32 + lane];
-                q4[0] = v.x; q4[1] = v.y; q4[2] = v.z; q4[3] = v.w;
-              } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) q4[e] = qf[nt][j][e];
-              }
-              mma16816(acc[nt], wa[j] & 0x000f000fu, wb[j] & 0x000f000fu, ya & 0x000f000fu,
-                       yb & 0x000f000fu, q4[0], q4[1]);
-              mma16816(acc[nt], wa[j] & 0x00f000f0u, wb[j] & 0x00f000f0u, ya & 0x00f000f0u,
-                       yb & 0x00f000f0u, q4[2], q4[3]);
+              for (int e = 0; e < 4; ++e) qv[nt][e] = qf[nt][j][e];
             }
           }
-          const float2 fa = __half22float2(as_h2(pa[g])), fb = __half22float2(as_h2(pb[g]));
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const uint32_t x0 = kw[u][0][j], x1 = kw[u][1][j], y0 = x0 >> 8, y1 = x1 >> 8;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              if (j == g * (GRP / 32))
+                mma16816_first(acc[u][nt], x0 & 0x000f000fu, x1 & 0x000f000fu, y0 & 0x000f000fu,
+                               y1 & 0x000f000fu, qv[nt][0], qv[nt][1]);
+              else
+                mma16816(acc[u][nt], x0 & 0x000f000fu, x1 & 0x000f000fu, y0 & 0x000f000fu,
+                         y1 & 0x000f000fu, qv[nt][0], qv[nt][1]);
+              mma16816(acc[u][nt], x0 & 0x00f000f0u, x1 & 0x00f000f0u, y0 & 0x00f000f0u,
+                       y1 & 0x00f000f0u, qv[nt][2], qv[nt][3]);
+            }
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float2 fa = __half22float2(as_h2(kp[u][0][g])), fb = __half22float2(as_h2(kp[u][1][g]));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float2 qs;
             if constexpr (X::GS) qs = reinterpret_cast<const float2*>(gsm)[(nt * NG + g) * 4 + c];
             else qs = f2(qsum[nt][g][0], qsum[nt][g][1]);
-            z[u][nt][0] = fmaf(fa.x, acc[nt][0], fmaf(fa.y, qs.x, z[u][nt][0]));
-            z[u][nt][1] = fmaf(fa.x, acc[nt][1], fmaf(fa.y, qs.y, z[u][nt][1]));
-            z[u][nt][2] = fmaf(fb.x, acc[nt][2], fmaf(fb.y, qs.x, z[u][nt][2]));
-            z[u][nt][3] = fmaf(fb.x, acc[nt][3], fmaf(fb.y, qs.y, z[u][nt][3]));
+            const float z0 = g ? z[u][nt][0] : 0.0f, z1 = g ? z[u][nt][1] : 0.0f;
+            const float z2 = g ? z[u][nt][2] : 0.0f, z3 = g ? z[u][nt][3] : 0.0f;
+            z[u][nt][0] = fmaf(fa.x, acc[u][nt][0], fmaf(fa.y, qs.x, z0));
+            z[u][nt][1] = fmaf(fa.x, acc[u][nt][1], fmaf(fa.y, qs.y, z1));
+            z[u][nt][2] = fmaf(fb.x, acc[u][nt][2], fmaf(fb.y, qs.x, z2));
+            z[u][nt][3] = fmaf(fb.x, acc[u][nt][3], fmaf(fb.y, qs.y, z3));
           }
         }
       }
@@ -479,7 +620,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
           top[nt][p] = fmaxf(v, m[nt][p]);
-          moved |= top[nt][p] > m[nt][p];
+          moved |= top[nt][p] > m[nt][p] + kPSlack;
         }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -549,146 +690,206 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
           }
       }
       __syncwarp();
-      if (next < t1) {
-        issue(next);
-        next += kAttnWarps;
-      }
+      if (getting) issue();
     }
-    if (timeout)  // nothing may land after the block has gone
-      for (; used < issued; ++used) mbar_wait(&full[warp][used % S], (used / S) & 1);
-    timeout = __syncthreads_or(timeout) != 0;
-    bad = __syncthreads_or(bad || timeout) != 0;
-    if (timeout && tid == 0) atomicAdd(&b2k_tu_timeouts, 1u);
-
-    // ---- the warps' parts meet (the rings are drained) ----------------------
-    float* mo = reinterpret_cast<float*>(smem);
+    if (timeout) break;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        float v = l[nt][p];
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
-        if (r == 0) {
-          mrg[warp][nt * 8 + 2 * c + p][0] = m[nt][p];
-          mrg[warp][nt * 8 + 2 * c + p][1] = v;
+        for (int x = 4; x < 32; x <<= 1) l[nt][p] += __shfl_xor_sync(0xffffffffu, l[nt][p], x);
+        if (bad) l[nt][p] = __int_as_float(0x7fc00000);
+      }
+    const bool whole = t0 == 0 && t1 == use.n;
+    const int64_t seg = (int64_t)use.entry * a.c.Hk + head;
+    if (t0 == 0 && lane == 0) {
+      // runs that hold the segment's first and last tile
+      const int64_t past = u1 - use.left - use.pos + use.n + kAttnLead;
+      a.spans[seg] = make_int2((int)run, whole ? (int)run : (int)run_of(past - 1));
+    }
+    if (one_segment) {  // the only part: the block's warps meet below
+      my_first = t0 == 0;
+      if (lane == 0) {
+        first_segment[0] = use.entry;  // the same from every warp
+        first_segment[1] = head;
+      }
+      my_last = t1 == use.n;
+      break;
+    }
+    const int64_t slot = 2 * run + (t0 == 0 ? 1 : 0);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int row = nt * 8 + 2 * c + p;
+        if (row0 + row >= R) continue;
+        if (whole) {
+          const int i = a.dG.div(row0 + row), hq = head * a.G + (row0 + row - i * a.G);
+          const float inv = attn_inverse(l[nt][p]);
+          uint16_t* dst = static_cast<uint16_t*>(a.o) +
+                          (((int64_t)b * a.Sq + i) * a.H + hq) * D + r * (D / 8);
+#pragma unroll
+          for (int k = 0; k < D / 64; ++k) {
+            const uint2 x = attn_pack4(make_float4(o[4 * k][nt][p], o[4 * k][nt][2 + p],
+                                                   o[4 * k + 1][nt][p], o[4 * k + 1][nt][2 + p]),
+                                       inv, a.bf16);
+            const uint2 y = attn_pack4(make_float4(o[4 * k + 2][nt][p], o[4 * k + 2][nt][2 + p],
+                                                   o[4 * k + 3][nt][p], o[4 * k + 3][nt][2 + p]),
+                                       inv, a.bf16);
+            *reinterpret_cast<uint4*>(dst + 8 * k) = make_uint4(x.x, x.y, y.x, y.y);
+          }
+          if (a.lse && r == 0)
+            a.lse[((int64_t)b * a.H + hq) * a.Sq + i] = attn_lse(m[nt][p], l[nt][p]);
+        } else {
+          float* dst = a.part + (slot * X::ROWS + row) * D + r * (D / 8);
+#pragma unroll
+          for (int k = 0; k < D / 32; ++k)
+            *reinterpret_cast<float4*>(dst + 4 * k) =
+                make_float4(o[2 * k][nt][p], o[2 * k][nt][2 + p], o[2 * k + 1][nt][p],
+                            o[2 * k + 1][nt][2 + p]);
+          if (r == 0) *attn_ml(a, slot * X::ROWS + row, X::ROWS * D) = make_float2(m[nt][p], l[nt][p]);
         }
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-          *reinterpret_cast<float2*>(mo + (size_t)(warp * X::ROWS + nt * 8 + 2 * c + p) * D +
-                                     r * (D / 8) + 2 * i) = f2(o[i][nt][p], o[i][nt][2 + p]);
       }
-    }
-    __syncthreads();
-    const bool whole = t0 == 0 && t1 == n_seg;
-    const int slot = (int)(2 * me + (t0 == 0 ? 1 : 0));
-    const int64_t seg = (int64_t)entry * a.c.Hk + head;
-    if (tid == 0 && t0 == 0) {
-      // blocks that hold the segment's first and last tile
-      const int64_t lastu = unit + n_seg - 1;
-      a.spans[seg] = make_int2((int)me, whole ? (int)me : (int)(((lastu + 1) * blocks - 1) / total));
-    }
-    for (int x = tid; x < X::ROWS * (D / 4); x += blockDim.x) {
-      const int row = x / (D / 4), d = (x - row * (D / 4)) * 4;
-      if (row0 + row >= R) continue;
-      float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kAttnWarps; ++w) M = fmaxf(M, mrg[w][row][0]);
-      float L = 0.0f;
-      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-      for (int w = 0; w < kAttnWarps; ++w) {
-        const float mw = mrg[w][row][0];
-        const float f = mw == -INFINITY ? (mrg[w][row][1] == 0.0f ? 0.0f : 1.0f) : ex2_approx(mw - M);
-        const float4 t = *reinterpret_cast<const float4*>(mo + (size_t)(w * X::ROWS + row) * D + d);
-        L = fmaf(mrg[w][row][1], f, L);
-        v.x = fmaf(t.x, f, v.x); v.y = fmaf(t.y, f, v.y);
-        v.z = fmaf(t.z, f, v.z); v.w = fmaf(t.w, f, v.w);
-      }
-      if (bad) L = __int_as_float(0x7fc00000);
-      if (!whole) {
-        *reinterpret_cast<float4*>(a.part + ((size_t)slot * X::ROWS + row) * D + d) = v;
-        if (d == 0) {
-          float* ml = a.part + (size_t)2 * gridDim.x * X::ROWS * D + ((size_t)slot * X::ROWS + row) * 2;
-          ml[0] = M;
-          ml[1] = L;
-        }
-        continue;
-      }
-      const int i = (row0 + row) / a.G, hq = head * a.G + (row0 + row - i * a.G);
-      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-      const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
-      const int64_t at = (((int64_t)b * a.Sq + i) * a.H + hq) * D + d;
-      uint2 w2;
-      if (a.bf16) {
-        __nv_bfloat162 p0 = __floats2bfloat162_rn(y[0], y[1]), p1 = __floats2bfloat162_rn(y[2], y[3]);
-        w2 = make_uint2(*reinterpret_cast<uint32_t*>(&p0), *reinterpret_cast<uint32_t*>(&p1));
-      } else {
-        w2 = make_uint2(as_u32(__floats2half2_rn(y[0], y[1])), as_u32(__floats2half2_rn(y[2], y[3])));
-      }
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = w2;
-      if (a.lse && d == 0)
-        a.lse[((int64_t)b * a.H + hq) * a.Sq + i] =
-            L == 0.0f ? -INFINITY : (M - kPScale) * kLn2 + logf(L);
-    }
-    __syncthreads();
+    attn_step(a, use);
+  }
+  if (timeout) {  // nothing may land after the block has gone
+    for (; used < issued; ++used) mbar_wait(&full[warp][used % S], (used / S) & 1);
+    if (lane == 0) atomicAdd(&b2k_tu_timeouts, 1u);
+  }
+  if (!one_segment) return;
 
-    unit += t1 - t0;
-    t0 = 0;
-    if (++head == a.c.Hk) {
-      head = 0;
-      ++entry;
-      if (unit < u1) n_seg = attn_tiles<D, NT>(a, entry);
+  // ---- the block's warps merge their parts of one segment ---------------------
+  if (lane == 0) ends[warp] = (my_first ? 1 : 0) | (my_last ? 2 : 0);
+  __syncthreads();  // the rings are drained: their memory holds the parts now
+  float* mo = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int row = nt * 8 + 2 * c + p;
+      if (r == 0) {
+        mrg[warp][row][0] = m[nt][p];
+        mrg[warp][row][1] = l[nt][p];
+      }
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+        *reinterpret_cast<float2*>(mo + (warp * X::ROWS + row) * D + r * (D / 8) + 2 * i) =
+            f2(o[i][nt][p], o[i][nt][2 + p]);
+    }
+  __syncthreads();
+  int first = -1, both = 0;  // the warp with the segment's first tile
+#pragma unroll
+  for (int w = 0; w < kAttnWarps; ++w) {
+    if (ends[w] & 1) first = w;
+    both |= ends[w];
+  }
+  const int entry = first_segment[0], head = first_segment[1];
+  const int b = a.dRT.div(entry), row0 = (entry - b * a.RT) * X::ROWS, R = (int)(a.Sq * a.G);
+  const int64_t slot = 2 * (run0 + max(first, 0)) + (first >= 0 ? 1 : 0);
+  if (both != 3 && tid < X::ROWS * kAttnWarps) {
+    // the other warps' slots, which the merge passes, hold nothing
+    const int w = tid / X::ROWS, row = tid - w * X::ROWS;
+    if (w > max(first, 0)) *attn_ml(a, 2 * (run0 + w) * X::ROWS + row, X::ROWS * D) = make_float2(-INFINITY, 0.0f);
+  }
+  for (int x = tid; x < X::ROWS * (D / 4); x += blockDim.x) {
+    const int row = x / (D / 4), d = (x - row * (D / 4)) * 4;
+    if (row0 + row >= R) continue;
+    float M = -INFINITY, L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kAttnWarps; ++w) M = fmaxf(M, mrg[w][row][0]);
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < kAttnWarps; ++w) {
+      const float f = attn_weight(mrg[w][row][0], mrg[w][row][1], M);
+      const float4 t = *reinterpret_cast<const float4*>(mo + (w * X::ROWS + row) * D + d);
+      L = fmaf(mrg[w][row][1], f, L);
+      v.x = fmaf(t.x, f, v.x); v.y = fmaf(t.y, f, v.y);
+      v.z = fmaf(t.z, f, v.z); v.w = fmaf(t.w, f, v.w);
+    }
+    if (both == 3) {
+      const int i = a.dG.div(row0 + row), hq = head * a.G + (row0 + row - i * a.G);
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) +
+                                (((int64_t)b * a.Sq + i) * a.H + hq) * D + d) =
+          attn_pack4(v, attn_inverse(L), a.bf16);
+      if (a.lse && d == 0) a.lse[((int64_t)b * a.H + hq) * a.Sq + i] = attn_lse(M, L);
+    } else {
+      *reinterpret_cast<float4*>(a.part + (slot * X::ROWS + row) * D + d) = v;
+      if (d == 0) *attn_ml(a, slot * X::ROWS + row, X::ROWS * D) = make_float2(M, L);
     }
   }
+  if (both == 3 && tid == 0) a.spans[(int64_t)entry * a.c.Hk + head] = make_int2(0, 0);
 }
 
-// Merges the partial (m, l, O) of segments that span blocks, in block order.
-// One block per row of a segment: D / 4 threads hold four dimensions each.
+// Merges the partial (m, l, O) of segments that span runs.  One block per row
+// of a segment: all threads read the parts' (m, l) at once and leave their
+// weights in shared memory, then D / 4 threads hold four dimensions each and
+// kMergeSlices such slices take every kMergeSlices-th part, their loads
+// independent of one another.  Fixed order of sums.
+constexpr int kMergeSlices = 8, kMergeChunk = 1024;
 template <int D, int NT>
-__global__ void __launch_bounds__(D / 4) kv4_attn_merge_kernel(const __grid_constant__ Kv4AttnArgs a,
-                                                                int blocks) {
-  constexpr int ROWS = attn_rows(NT);
+__global__ void __launch_bounds__(D / 4 * kMergeSlices) kv4_attn_merge_kernel(
+    const __grid_constant__ Kv4AttnArgs a) {
+  constexpr int ROWS = attn_rows(NT), THREADS = D / 4 * kMergeSlices;
+  __shared__ float4 sv[kMergeSlices][D / 4];
+  __shared__ float weight[kMergeChunk], red[2][THREADS / 32];
   griddep_launch_dependents();
   griddep_wait();
   const int64_t seg = blockIdx.x;
-  const int row = blockIdx.y, d = threadIdx.x * 4;
+  const int row = blockIdx.y, tid = threadIdx.x, slice = tid / (D / 4), d4 = tid - slice * (D / 4);
   const int2 span = a.spans[seg];
   if (span.x == span.y) return;
-  const int64_t entry = seg / a.c.Hk, b = entry / a.RT;
-  const int head = (int)(seg - entry * a.c.Hk);
-  const int64_t rr = (entry - b * a.RT) * ROWS + row;
-  if (rr >= a.Sq * a.G) return;
-  const float* ml = a.part + (size_t)2 * blocks * ROWS * D;
-  float M = -INFINITY, L = 0.0f;
+  const int entry = a.dHk.div((int)seg), b = a.dRT.div(entry), head = (int)seg - entry * a.c.Hk;
+  const int rr = (entry - b * a.RT) * ROWS + row, parts = span.y - span.x + 1;
+  if (rr >= (int)(a.Sq * a.G)) return;
+  auto slot = [&](int i) { return (2 * (int64_t)(span.x + i) + (i == 0 ? 1 : 0)) * ROWS + row; };
+  float M = -INFINITY;
+  for (int i = tid; i < parts; i += THREADS) M = fmaxf(M, attn_ml(a, slot(i), ROWS * D)->x);
+  M = warp_allmax(M);
+  if ((tid & 31) == 0) red[0][tid >> 5] = M;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) M = fmaxf(M, red[0][w]);
+  float L = 0.0f;
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int i = span.x; i <= span.y; ++i) {
-    const size_t slot = (size_t)(2 * i + (i == span.x ? 1 : 0)) * ROWS + row;
-    const float2 p = *reinterpret_cast<const float2*>(ml + 2 * slot);
-    const float4 t = *reinterpret_cast<const float4*>(a.part + slot * D + d);
-    const float Mn = fmaxf(M, p.x);
-    const float f0 = M == -INFINITY ? (L == 0.0f ? 0.0f : 1.0f) : ex2_approx(M - Mn);
-    const float f1 = p.x == -INFINITY ? (p.y == 0.0f ? 0.0f : 1.0f) : ex2_approx(p.x - Mn);
-    L = L * f0 + p.y * f1;
-    v.x = v.x * f0 + t.x * f1; v.y = v.y * f0 + t.y * f1;
-    v.z = v.z * f0 + t.z * f1; v.w = v.w * f0 + t.w * f1;
-    M = Mn;
+  for (int base = 0; base < parts; base += kMergeChunk) {
+    const int n = min(parts - base, kMergeChunk);
+    __syncthreads();
+    for (int i = tid; i < n; i += THREADS) {
+      const float2 p = *attn_ml(a, slot(base + i), ROWS * D);
+      const float f = attn_weight(p.x, p.y, M);
+      weight[i] = f;
+      L = fmaf(p.y, f, L);
+    }
+    __syncthreads();
+#pragma unroll 8
+    for (int i = slice; i < n; i += kMergeSlices) {
+      const float f = weight[i];
+      if (f != 0.0f) {  // a part that holds nothing has no output either
+        const float4 t = *reinterpret_cast<const float4*>(a.part + slot(base + i) * D + 4 * d4);
+        v.x = fmaf(t.x, f, v.x); v.y = fmaf(t.y, f, v.y);
+        v.z = fmaf(t.z, f, v.z); v.w = fmaf(t.w, f, v.w);
+      }
+    }
   }
-  const int64_t i = rr / a.G, hq = head * a.G + (rr - i * a.G);
-  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-  const int64_t at = ((b * a.Sq + i) * a.H + hq) * D + d;
-  uint2 w2;
-  if (a.bf16) {
-    __nv_bfloat162 p0 = __floats2bfloat162_rn(v.x * inv, v.y * inv);
-    __nv_bfloat162 p1 = __floats2bfloat162_rn(v.z * inv, v.w * inv);
-    w2 = make_uint2(*reinterpret_cast<uint32_t*>(&p0), *reinterpret_cast<uint32_t*>(&p1));
-  } else {
-    w2 = make_uint2(as_u32(__floats2half2_rn(v.x * inv, v.y * inv)),
-                    as_u32(__floats2half2_rn(v.z * inv, v.w * inv)));
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+  if ((tid & 31) == 0) red[1][tid >> 5] = L;
+  sv[slice][d4] = v;
+  __syncthreads();
+  if (slice) return;
+  L = 0.0f;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) L += red[1][w];
+#pragma unroll
+  for (int s = 1; s < kMergeSlices; ++s) {
+    const float4 t = sv[s][d4];
+    v.x += t.x; v.y += t.y; v.z += t.z; v.w += t.w;
   }
-  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + at) = w2;
-  if (a.lse && d == 0)
-    a.lse[(b * a.H + hq) * a.Sq + i] = L == 0.0f ? -INFINITY : (M - kPScale) * kLn2 + logf(L);
+  const int i = a.dG.div(rr), hq = head * a.G + (rr - i * a.G);
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + (((int64_t)b * a.Sq + i) * a.H + hq) * D +
+                            4 * d4) = attn_pack4(v, attn_inverse(L), a.bf16);
+  if (a.lse && d4 == 0) a.lse[((int64_t)b * a.H + hq) * a.Sq + i] = attn_lse(M, L);
 }
 
 // columns of the products, in eights: the fewest that hold the rows, up to
@@ -700,7 +901,7 @@ static int attn_nt(int64_t rows, int64_t D) {
 }
 
 struct AttnPlan {
-  int nt, blocks;
+  int nt, blocks, warps;
   int64_t rt, segs, part_bytes, bytes;
 };
 
@@ -710,8 +911,9 @@ static AttnPlan attn_plan(int64_t B, int64_t Sq, int64_t H, int64_t Hk, int64_t 
   p.nt = attn_nt(rows, D);
   p.rt = (rows + 8 * p.nt - 1) / (8 * p.nt);
   p.blocks = sm_count() * attn_cps((int)D, p.nt);
+  p.warps = p.blocks * kAttnWarps;
   p.segs = B * p.rt * Hk;
-  p.part_bytes = (int64_t)2 * p.blocks * 8 * p.nt * (D + 2) * 4;
+  p.part_bytes = (int64_t)2 * p.warps * 8 * p.nt * (D + 2) * 4;
   p.bytes = p.part_bytes + p.segs * (int64_t)sizeof(int2);
   return p;
 }
@@ -728,8 +930,8 @@ static int attn_launch(const Kv4AttnArgs& a, const AttnPlan& p, cudaStream_t st)
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
   launch_pdl(kern, dim3(p.blocks), dim3(32 * kAttnWarps), AttnShape<D, GRP, NT>::SMEM, st, a);
-  launch_pdl(kv4_attn_merge_kernel<D, NT>, dim3((unsigned)p.segs, 8 * NT), dim3(D / 4), 0, st, a,
-             p.blocks);
+  launch_pdl(kv4_attn_merge_kernel<D, NT>, dim3((unsigned)p.segs, 8 * NT), dim3(D / 4 * kMergeSlices), 0,
+             st, a);
   return check_launch("b2k_kv4_attention");
 }
 
@@ -774,7 +976,7 @@ extern "C" int b2k_kv4_attention(const void* q, int64_t qb, int64_t qs, int64_t 
   B2K_REQUIRE(width <= (0x7fffffffLL - 64) / P, "b2k_kv4_attention: a table of %lld pages is too wide",
               (long long)width);
   B2K_REQUIRE(q && o && lens && (table || width == 0), "b2k_kv4_attention: null operand");
-  B2K_REQUIRE((reinterpret_cast<uintptr_t>(o) & 7u) == 0, "b2k_kv4_attention: o is not 8-byte aligned");
+  B2K_REQUIRE(aligned16(o), "b2k_kv4_attention: o is not 16-byte aligned");
   const AttnPlan p = attn_plan(B, Sq, H, Hk, D);
   B2K_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= p.bytes,
               "b2k_kv4_attention: the workspace needs %lld aligned bytes, got %lld",
@@ -789,6 +991,11 @@ extern "C" int b2k_kv4_attention(const void* q, int64_t qb, int64_t qs, int64_t 
   a.q_aligned = aligned16(q) && qb % 8 == 0 && qs % 8 == 0 && qh % 8 == 0;
   a.G = (int)(H / Hk);
   a.RT = (int)p.rt;
+  a.warps = p.warps;
+  a.dG = fast_div(a.G);
+  a.dRT = fast_div(a.RT);
+  a.dP = fast_div(P);
+  a.dHk = fast_div(Hk);
   a.part = static_cast<float*>(workspace);
   a.spans = reinterpret_cast<int2*>(static_cast<unsigned char*>(workspace) + p.part_bytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
