@@ -94,12 +94,9 @@ struct Kv4AttnArgs {
   int2* spans;      // [segments] first and last warp
 };
 
-// tokens of a tile: about the same bytes for every D, and registers for its
-// scores (NT T / 8 per thread) beside the output's
-__host__ __device__ constexpr int attn_tile(int D, int NT) { return D == 256 || NT * D > 256 ? 16 : 32; }
 __host__ __device__ constexpr int attn_rows(int NT) { return 8 * NT; }
 // resident blocks per SM: registers (NT D / 4 for the output) and shared memory
-__host__ __device__ constexpr int attn_cps(int D, int NT) { return NT * D > 256 ? 2 : 3; }
+__host__ __device__ constexpr int attn_cps(int D, int NT) { return NT * D >= 256 && NT > 1 ? 2 : 3; }
 
 // Token counts fit 32 bits (the host refuses wider tables), runs of tiles over
 // all segments do not.
@@ -115,10 +112,10 @@ __device__ __forceinline__ int attn_end(const Kv4AttnArgs& a, int len, int rt) {
   return max(a.causal ? len - (int)a.Sq + a.dG.div(last_row) + 1 : len, 0);
 }
 // tiles of each of its segments (one at least: somebody writes the zeros)
-template <int D, int NT> __device__ __forceinline__ int attn_tiles(const Kv4AttnArgs& a, int entry) {
+template <int D, int NT, int T> __device__ __forceinline__ int attn_tiles(const Kv4AttnArgs& a, int entry) {
   bool bad;
   const int b = a.dRT.div(entry), end = attn_end<D, NT>(a, attn_len(a, b, bad), entry - b * a.RT);
-  return max((end + attn_tile(D, NT) - 1) / attn_tile(D, NT), 1);
+  return max((end + T - 1) / T, 1);
 }
 
 __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2,
@@ -161,32 +158,43 @@ template <int BYTES> __device__ __forceinline__ void load_words(uint32_t* w, con
   }
 }
 
+// A constant that stays in its register (the compiler would otherwise build it
+// anew before most uses).
+__device__ __forceinline__ uint32_t held(uint32_t v) {
+  uint32_t r;
+  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+struct ValueConsts {
+  uint32_t magic;        // 0x6400 in both halves: 0x6400 | n is 1024 + n
+  __half2 sixteenth, m64;
+};
+
 // four nibbles of each half of x (the halves: two tokens) -> (lo + s n) pairs
-__device__ __forceinline__ void value_pairs(uint32_t x, __half2 s, __half2 lo, uint32_t* out) {
-  const __half2 k1024 = __float2half2_rn(1024.0f), k16 = __float2half2_rn(0.0625f),
-                km64 = __float2half2_rn(-64.0f);
+__device__ __forceinline__ void value_pairs(uint32_t x, __half2 s, __half2 lo, const ValueConsts& k,
+                                            uint32_t* out) {
+  const __half2 m1024 = __float2half2_rn(-1024.0f);
   const uint32_t y = x >> 8;
-  // 0x6400 | n is 1024 + n; the upper nibble of a byte is 1024 + 16 n
-  const __half2 n0 = __hsub2(as_h2((x & 0x000f000fu) | 0x64006400u), k1024);
-  const __half2 n1 = __hfma2(as_h2((x & 0x00f000f0u) | 0x64006400u), k16, km64);
-  const __half2 n2 = __hsub2(as_h2((y & 0x000f000fu) | 0x64006400u), k1024);
-  const __half2 n3 = __hfma2(as_h2((y & 0x00f000f0u) | 0x64006400u), k16, km64);
+  // the upper nibble of a byte comes as 1024 + 16 n
+  const __half2 n0 = __hadd2(as_h2((x & 0x000f000fu) | k.magic), m1024);
+  const __half2 n1 = __hfma2(as_h2((x & 0x00f000f0u) | k.magic), k.sixteenth, k.m64);
+  const __half2 n2 = __hadd2(as_h2((y & 0x000f000fu) | k.magic), m1024);
+  const __half2 n3 = __hfma2(as_h2((y & 0x00f000f0u) | k.magic), k.sixteenth, k.m64);
   out[0] = as_u32(__hfma2(n0, s, lo));
   out[1] = as_u32(__hfma2(n1, s, lo));
   out[2] = as_u32(__hfma2(n2, s, lo));
   out[3] = as_u32(__hfma2(n3, s, lo));
 }
 
-template <int D, int GRP, int NT> struct AttnShape {
-  static constexpr int T = attn_tile(D, NT), U = T / 16, J = D / 32, NG = D / GRP, ROWS = attn_rows(NT);
+template <int D, int GRP, int NT, int T> struct AttnShape {
+  static constexpr int U = T / 16, J = D / 32, NG = D / GRP, ROWS = attn_rows(NT);
   static constexpr int MB = 16 * (D + 8 * NG);           // bytes of a micro block
   static constexpr int KP = 8 * D, VR = KP + 64 * NG, VP = VR + 8 * D;  // its fields
   static constexpr int STAGE = U * MB;
   static constexpr int MERGE = kAttnWarps * ROWS * D * 4;
-  // query fragments, and the groups' sums, in shared memory instead of registers
-  static constexpr bool QS = NT * D > 128, GS = NT * NG > 4;
-  static constexpr int QB = QS ? NT * J * 512 : 0;
-  static constexpr int WARP = kAttnStages * STAGE + QB + (GS ? NT * NG * 32 : 0);
+  // each warp's shared memory: its ring, the fragments of its queries and their
+  // sums over each group
+  static constexpr int QB = NT * J * 512, WARP = kAttnStages * STAGE + QB + NT * NG * 32;
   static constexpr int SMEM = kAttnWarps * WARP > MERGE ? kAttnWarps * WARP : MERGE;
 };
 
@@ -223,9 +231,10 @@ struct AttnWalk {
   int t, t1;
 };
 // on to the next part that has tiles
-template <int D, int NT> __device__ __forceinline__ bool attn_next(const Kv4AttnArgs& a, AttnWalk& k) {
+template <int D, int NT, int T>
+__device__ __forceinline__ bool attn_next(const Kv4AttnArgs& a, AttnWalk& k) {
   while (k.left > 0) {
-    if (k.n == 0) k.n = attn_tiles<D, NT>(a, k.entry);
+    if (k.n == 0) k.n = attn_tiles<D, NT, T>(a, k.entry);
     const int take = min(k.left, k.n + kAttnLead - k.pos);
     k.t = max(k.pos - kAttnLead, 0);
     k.t1 = max(k.pos + take - kAttnLead, 0);
@@ -247,11 +256,11 @@ __device__ __forceinline__ void attn_step(const Kv4AttnArgs& a, AttnWalk& k) {
   }
 }
 
-template <int D, int GRP, int NT>
+template <int D, int GRP, int NT, int T>
 __global__ void __launch_bounds__(32 * kAttnWarps, attn_cps(D, NT))
 kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
-  using X = AttnShape<D, GRP, NT>;
-  constexpr int T = X::T, U = X::U, J = X::J, NG = X::NG, MB = X::MB, S = kAttnStages;
+  using X = AttnShape<D, GRP, NT, T>;
+  constexpr int U = X::U, J = X::J, NG = X::NG, MB = X::MB, S = kAttnStages;
   constexpr int VW = D / 64;  // words of a lane's D / 8 value dimensions
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint64_t full[kAttnWarps][S];
@@ -272,7 +281,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
   const int chunk = (entries + 31) / 32;
   const int e0 = min(entries, lane * chunk), e1 = min(entries, e0 + chunk);
   int64_t mine = 0;
-  for (int e = e0; e < e1; ++e) mine += attn_tiles<D, NT>(a, e) + kAttnLead;
+  for (int e = e0; e < e1; ++e) mine += attn_tiles<D, NT, T>(a, e) + kAttnLead;
   int64_t before = mine;
 #pragma unroll
   for (int x = 1; x < 32; x <<= 1) {
@@ -303,7 +312,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
     int e = e0, n = 0;
     if (here)
       for (;; ++e) {
-        n = attn_tiles<D, NT>(a, e);
+        n = attn_tiles<D, NT, T>(a, e);
         const int64_t all = (int64_t)(n + kAttnLead) * a.c.Hk;
         if (at < all) break;
         at -= all;
@@ -322,62 +331,70 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
   // the warps past the last run join the merge of the others
   one_segment = __syncthreads_or(one_segment) != 0;
   AttnWalk get = use;
-  uint32_t issued = 0, used = 0;  // stages
+  uint32_t issued = 0, used = 0, use_phase = 0;  // tiles
+  int use_stage = 0;
   bool timeout = false;
 
   // ---- the ring: the walk `get` runs ahead of `use` by up to S tiles ---------
-  // lane l < U fetches the 16 tokens from `get_tok` of its page, which it looked
-  // up one tile before
-  int get_tok = 0, get_off = 0, get_end = 0, get_pid = 0;
+  // A tile lies within a page.  get_src: its bytes, for as long as the page (or
+  // the part) lasts, up to tile get_stop; a page is looked up one call before
+  // it is needed.
+  int get_stop = 0, get_end = 0, get_pid = 0, get_at = 0, get_stage = 0;
   const int32_t* get_page = nullptr;
-  bool getting = false, bad = false, my_first = false, my_last = false;
-  uint32_t bad_stages = 0;  // a page outside the pool among the tokens of a stage
+  const unsigned char* get_src = nullptr;
+  bool getting = false, get_fresh = false, get_ok = false;
+  bool bad = false, my_first = false, my_last = false;
+  uint32_t bad_stages = 0;  // stages of tokens whose page is outside the pool
   const int64_t head_bytes = (int64_t)(a.c.P >> 4) * MB;
   auto open = [&]() {  // the next part's first tile
-    getting = attn_next<D, NT>(a, get);
+    getting = attn_next<D, NT, T>(a, get);
     if (getting) {
-      const int b = a.dRT.div(get.entry);
+      const int b = a.dRT.div(get.entry), tok = get.t * T, pi = a.dP.div(tok);
       bool over;
-      get_end = lane < U ? attn_end<D, NT>(a, attn_len(a, b, over), get.entry - b * a.RT) : 0;
-      get_tok = get.t * T + (lane < U ? 16 * lane : 0);
-      const int pi = a.dP.div(get_tok);
+      get_end = attn_end<D, NT>(a, attn_len(a, b, over), get.entry - b * a.RT);
       get_page = a.table + b * a.width + pi;
-      get_off = get_tok - pi * a.c.P;
-      get_pid = get_tok < get_end ? *get_page : -1;
+      get_pid = get_end > 0 ? *get_page : -1;
+      get_at = tok - pi * a.c.P;
+      get_stop = min(get.t1, get.t + (a.c.P - get_at) / T);
+      get_fresh = true;
     }
   };
   auto issue = [&]() {
-    const int s = issued % S;
-    const bool have = get_tok < get_end && get_pid >= 0 && get_pid < a.c.pages;
-    const uint32_t got = __ballot_sync(0xffffffffu, have);
-    const uint32_t miss = __any_sync(0xffffffffu, get_tok < get_end && !have) ? 1u : 0u;
-    bad_stages = (bad_stages & ~(1u << s)) | (miss << s);
-    fence_proxy_async();
-    if (lane == 0) mbar_arrive_expect_tx(&full[warp][s], __popc(got) * MB);
-    __syncwarp();
-    if (have)
-      bulk_g2s(ring + s * X::STAGE + lane * MB,
-               a.c.data + ((int64_t)get_pid * a.c.Hk + get.head) * head_bytes + (get_off >> 4) * MB, MB,
-               &full[warp][s]);
+    if (get_fresh) {
+      get_fresh = false;
+      get_ok = (uint32_t)get_pid < (uint32_t)a.c.pages;
+      get_src = a.c.data + ((int64_t)get_pid * a.c.Hk + get.head) * head_bytes + (get_at >> 4) * MB;
+    }
+    if (lane == 0) {
+      uint64_t* bar = &full[warp][get_stage];
+      fence_proxy_async();
+      mbar_arrive_expect_tx(bar, get_ok ? X::STAGE : 0);
+      if (get_ok) bulk_g2s(ring + get_stage * X::STAGE, get_src, X::STAGE, bar);
+    }
+    get_src += X::STAGE;
+    if (!get_ok || bad_stages)
+      bad_stages = (bad_stages & ~(1u << get_stage)) | ((uint32_t)(!get_ok && get_end > 0) << get_stage);
+    if (++get_stage == S) get_stage = 0;
     ++issued;
-    if (++get.t == get.t1) {
-      attn_step(a, get);
-      open();
-    } else {
-      get_tok += T;
-      get_off += T;
-      while (get_off >= a.c.P) {
-        get_off -= a.c.P;
-        ++get_page;
+    if (++get.t == get_stop) {
+      if (get.t == get.t1) {
+        attn_step(a, get);
+        open();
+      } else {
+        get_pid = *++get_page;
+        get_at = 0;
+        get_stop = min(get.t1, get_stop + a.c.P / T);
+        get_fresh = true;
       }
-      get_pid = get_tok < get_end ? *get_page : -1;
     }
   };
   open();
   for (int k = 0; k < S && getting; ++k) issue();
 
+  const ValueConsts vk = {held(0x64006400u), as_h2(held(0x2c002c00u)), as_h2(held(0xd400d400u))};
+  // per row: maximum, sum, score that moves the maximum, exponent's offset
   float o[D / 16][NT][4];
-  float m[NT][2], l[NT][2];
+  float m[NT][2], l[NT][2], lim[NT][2], off[NT][2];
   auto clear = [&]() {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -386,12 +403,13 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.0f;
       m[nt][0] = m[nt][1] = -INFINITY;
-      l[nt][0] = l[nt][1] = 0.0f;
+      l[nt][0] = l[nt][1] = off[nt][0] = off[nt][1] = 0.0f;
+      lim[nt][0] = lim[nt][1] = -INFINITY;
     }
   };
   clear();
 
-  while (!timeout && attn_next<D, NT>(a, use)) {
+  while (!timeout && attn_next<D, NT, T>(a, use)) {
     const int b = a.dRT.div(use.entry), rt = use.entry - b * a.RT, head = use.head;
     const int t0 = use.t, t1 = use.t1;
     const int len = attn_len(a, b, bad);
@@ -405,9 +423,8 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
 
     // ---- query rows -> B fragments -----------------------------------------
     // lane (r, c) holds row r of each 8, dimensions 32 j + 8 c .. + 7
-    uint32_t qf[X::QS ? 1 : NT][X::QS ? 1 : J][4];
-    float qsum[X::GS ? 1 : NT][X::GS ? 1 : NG][2], cmul[NT][2];
-    if (X::QS || X::GS) __syncwarp();
+    float cmul[NT][2];
+    __syncwarp();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int row = row0 + nt * 8 + r;
@@ -439,8 +456,9 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // 2^(9 - floor(log2 top)); 1 for a row of zeros or one that is not finite
       const int ex = (int)(__float_as_uint(top) >> 23);
-      const float f = top > 0.0f && ex < 255
-                          ? __uint_as_float((uint32_t)min(263 - ex, 254) << 23) : 1.0f;
+      const float mag = top > 0.0f && ex < 255
+                            ? __uint_as_float((uint32_t)min(263 - ex, 254) << 23) : 1.0f;
+      const float f = a.scale < 0.0f ? -mag : mag;  // scores are multiplied by |scale|
       float part[NG];
 #pragma unroll
       for (int g = 0; g < NG; ++g) part[g] = 0.0f;
@@ -456,14 +474,10 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
         }
         uint32_t w[4] = {as_u32(__halves2half2(h[0], h[4])), as_u32(__halves2half2(h[2], h[6])),
                          as_u32(__halves2half2(h[1], h[5])), as_u32(__halves2half2(h[3], h[7]))};
-        if constexpr (X::QS) {
-          reinterpret_cast<uint4*>(qsm)[(nt * J + j) * 32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) qf[nt][j][e] = w[e];
-        }
+        reinterpret_cast<uint4*>(qsm)[(nt * J + j) * 32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      const float cm = a.scale * kLog2e * (16777216.0f / f);
+      // at least a number that leaves scale = 0 a factor of its own: 0 * -inf is NaN
+      const float cm = fmaxf(fabsf(a.scale) * kLog2e * (16777216.0f / mag), 1e-37f);
 #pragma unroll
       for (int p = 0; p < 2; ++p) {  // what this lane's columns 2c, 2c + 1 need
         const int src = (2 * c + p) * 4;
@@ -475,30 +489,30 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
         t += __shfl_xor_sync(0xffffffffu, t, 1);
         t += __shfl_xor_sync(0xffffffffu, t, 2);
         t *= 5.9604644775390625e-8f;  // 2^-24, the unit of the integers' products
-        if constexpr (X::GS) {
-          if (c == 0) gsm[(nt * NG + g) * 8 + r] = t;
-        } else {
-          qsum[nt][g][0] = __shfl_sync(0xffffffffu, t, 8 * c);
-          qsum[nt][g][1] = __shfl_sync(0xffffffffu, t, 8 * c + 4);
-        }
+        if (c == 0) gsm[(nt * NG + g) * 8 + r] = t;
       }
     }
-    if (X::QS || X::GS) __syncwarp();
+    __syncwarp();
     const int all_see = last_of(0);  // tokens up to here are seen by every row
+    const int mask_from = max(all_see + 1, 0) / T;  // and the tiles before this one
 
     clear();
 
     for (int t = t0; t < t1; ++t) {
-      const int s = used % S;
-      if (!mbar_wait(&full[warp][s], (used / S) & 1)) {
+      const int s = use_stage;
+      if (!mbar_wait(&full[warp][s], use_phase)) {
         timeout = true;
         break;
       }
       ++used;
-      bad |= (bad_stages >> s) & 1;
+      if (++use_stage == S) {
+        use_stage = 0;
+        use_phase ^= 1;
+      }
+      if (bad_stages) bad |= (bad_stages >> s) & 1;
       unsigned char* st = ring + s * X::STAGE;
       const int tok0 = t * T;
-      const bool masked = tok0 + T - 1 > all_see;
+      const bool masked = t >= mask_from;
       if (masked) {
         // What lies past the length is garbage, and a value some row does not
         // see must not reach it as 0 * NaN: such parameters become zero, and
@@ -537,7 +551,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const unsigned char* mb = st + u * MB;
+          const unsigned char* mb = st + (u) * MB;
           load_words<D / 8>(kw[u][h], mb + (r + 8 * h) * (D / 2) + c * (D / 8));
           load_words<4 * NG>(kp[u][h], mb + X::KP + (r + 8 * h) * 4 * NG);
         }
@@ -549,13 +563,8 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
           uint32_t qv[NT][4];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            if constexpr (X::QS) {
-              const uint4 v = reinterpret_cast<const uint4*>(qsm)[(nt * J + j) * 32 + lane];
-              qv[nt][0] = v.x; qv[nt][1] = v.y; qv[nt][2] = v.z; qv[nt][3] = v.w;
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) qv[nt][e] = qf[nt][j][e];
-            }
+            const uint4 v = reinterpret_cast<const uint4*>(qsm)[(nt * J + j) * 32 + lane];
+            qv[nt][0] = v.x; qv[nt][1] = v.y; qv[nt][2] = v.z; qv[nt][3] = v.w;
           }
 #pragma unroll
           for (int u = 0; u < U; ++u) {
@@ -578,60 +587,55 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
           const float2 fa = __half22float2(as_h2(kp[u][0][g])), fb = __half22float2(as_h2(kp[u][1][g]));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float2 qs;
-            if constexpr (X::GS) qs = reinterpret_cast<const float2*>(gsm)[(nt * NG + g) * 4 + c];
-            else qs = f2(qsum[nt][g][0], qsum[nt][g][1]);
-            const float z0 = g ? z[u][nt][0] : 0.0f, z1 = g ? z[u][nt][1] : 0.0f;
-            const float z2 = g ? z[u][nt][2] : 0.0f, z3 = g ? z[u][nt][3] : 0.0f;
-            z[u][nt][0] = fmaf(fa.x, acc[u][nt][0], fmaf(fa.y, qs.x, z0));
-            z[u][nt][1] = fmaf(fa.x, acc[u][nt][1], fmaf(fa.y, qs.y, z1));
-            z[u][nt][2] = fmaf(fb.x, acc[u][nt][2], fmaf(fb.y, qs.x, z2));
-            z[u][nt][3] = fmaf(fb.x, acc[u][nt][3], fmaf(fb.y, qs.y, z3));
+            const float2 qs = reinterpret_cast<const float2*>(gsm)[(nt * NG + g) * 4 + c];
+            float* zz = z[u][nt];
+            zz[0] = fmaf(fa.x, acc[u][nt][0], fmaf(fa.y, qs.x, g ? zz[0] : 0.0f));
+            zz[1] = fmaf(fa.x, acc[u][nt][1], fmaf(fa.y, qs.y, g ? zz[1] : 0.0f));
+            zz[2] = fmaf(fb.x, acc[u][nt][2], fmaf(fb.y, qs.x, g ? zz[2] : 0.0f));
+            zz[3] = fmaf(fb.x, acc[u][nt][3], fmaf(fb.y, qs.y, g ? zz[3] : 0.0f));
           }
         }
       }
 
       // ---- softmax: columns 2c, 2c + 1 are this lane's rows of queries -------
-      float top[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        top[nt][0] = top[nt][1] = -INFINITY;
-        int last[2] = {0, 0};
-        if (masked) {
-          last[0] = last_of(nt * 8 + 2 * c);
-          last[1] = last_of(nt * 8 + 2 * c + 1);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float v = z[u][nt][e] * cmul[nt][e & 1];
-            if (masked && tok0 + 16 * u + r + 8 * (e >> 1) > last[e & 1]) v = -INFINITY;
-            z[u][nt][e] = v;
-            top[nt][e & 1] = fmaxf(top[nt][e & 1], v);
-          }
-      }
+      // m is the maximum of the scores as they are; a tile moves it only when one
+      // is beyond it by more than the slack, which each lane checks for its own
       bool moved = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        if (masked) {
+          const int last[2] = {last_of(nt * 8 + 2 * c), last_of(nt * 8 + 2 * c + 1)};
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (tok0 + 16 * u + r + 8 * (e >> 1) > last[e & 1]) z[u][nt][e] = -INFINITY;
+        }
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          float v = top[nt][p];
+          float v = fmaxf(z[0][nt][p], z[0][nt][2 + p]);
 #pragma unroll
-          for (int x = 4; x < 32; x <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
-          top[nt][p] = fmaxf(v, m[nt][p]);
-          moved |= top[nt][p] > m[nt][p] + kPSlack;
+          for (int u = 1; u < U; ++u) v = fmaxf(v, fmaxf(z[u][nt][p], z[u][nt][2 + p]));
+          moved |= v > lim[nt][p];
         }
+      }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float f[2];
 #pragma unroll
           for (int p = 0; p < 2; ++p) {
+            float v = m[nt][p];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v = fmaxf(v, fmaxf(z[u][nt][p], z[u][nt][2 + p]));
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
             // from -inf: nothing was summed yet (0 * 0 whatever the new one is)
-            f[p] = m[nt][p] == -INFINITY ? 0.0f : ex2_approx(m[nt][p] - top[nt][p]);
+            f[p] = m[nt][p] == -INFINITY ? 0.0f : ex2_approx((m[nt][p] - v) * cmul[nt][p]);
             l[nt][p] *= f[p];
-            m[nt][p] = top[nt][p];
+            m[nt][p] = v;
+            lim[nt][p] = v + kPSlack / cmul[nt][p];
+            off[nt][p] = v == -INFINITY ? 0.0f : kPScale - v * cmul[nt][p];
           }
 #pragma unroll
           for (int i = 0; i < D / 16; ++i)
@@ -641,22 +645,18 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
       }
       uint32_t pf[U][NT][2];  // probabilities as B fragments: [tokens] x [rows]
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float off[2];
-#pragma unroll
-        for (int p = 0; p < 2; ++p) off[p] = m[nt][p] == -INFINITY ? 0.0f : m[nt][p] - kPScale;
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           float p[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            p[e] = ex2_approx(z[u][nt][e] - off[e & 1]);
+            p[e] = ex2_approx(fmaf(z[u][nt][e], cmul[nt][e & 1], off[nt][e & 1]));
             l[nt][e & 1] += p[e];
           }
           pf[u][nt][0] = transpose8x8(as_u32(__floats2half2_rn(p[0], p[1])));
           pf[u][nt][1] = transpose8x8(as_u32(__floats2half2_rn(p[2], p[3])));
         }
-      }
 
       // ---- output: [dimensions] x [rows] -----------------------------------
 #pragma unroll
@@ -679,8 +679,8 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
           for (int hi = 0; hi < 2; ++hi) {
             const uint32_t sel = hi ? 0x7632 : 0x5410;
             uint32_t x0[4], x1[4];
-            value_pairs(__byte_perm(v[0][w], v[1][w], sel), s0, o0, x0);
-            value_pairs(__byte_perm(v[2][w], v[3][w], sel), s1, o1, x1);
+            value_pairs(__byte_perm(v[0][w], v[1][w], sel), s0, o0, vk, x0);
+            value_pairs(__byte_perm(v[2][w], v[3][w], sel), s1, o1, vk, x1);
 #pragma unroll
             for (int q = 0; q < 2; ++q)
 #pragma unroll
@@ -700,6 +700,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l[nt][p] += __shfl_xor_sync(0xffffffffu, l[nt][p], x);
         if (bad) l[nt][p] = __int_as_float(0x7fc00000);
+        m[nt][p] *= cmul[nt][p];  // in powers of two from here on
       }
     const bool whole = t0 == 0 && t1 == use.n;
     const int64_t seg = (int64_t)use.entry * a.c.Hk + head;
@@ -918,30 +919,41 @@ static AttnPlan attn_plan(int64_t B, int64_t Sq, int64_t H, int64_t Hk, int64_t 
   return p;
 }
 
-template <int D, int GRP, int NT>
+template <int D, int GRP, int NT, int T>
 static int attn_launch(const Kv4AttnArgs& a, const AttnPlan& p, cudaStream_t st) {
-  auto kern = kv4_attn_kernel<D, GRP, NT>;
+  auto kern = kv4_attn_kernel<D, GRP, NT, T>;
   static bool done[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !done[dev]) {
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         AttnShape<D, GRP, NT>::SMEM);
+                         AttnShape<D, GRP, NT, T>::SMEM);
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
-  launch_pdl(kern, dim3(p.blocks), dim3(32 * kAttnWarps), AttnShape<D, GRP, NT>::SMEM, st, a);
+  launch_pdl(kern, dim3(p.blocks), dim3(32 * kAttnWarps), AttnShape<D, GRP, NT, T>::SMEM, st, a);
   launch_pdl(kv4_attn_merge_kernel<D, NT>, dim3((unsigned)p.segs, 8 * NT), dim3(D / 4 * kMergeSlices), 0,
              st, a);
   return check_launch("b2k_kv4_attention");
 }
 
+// Tiles of 32 tokens where pages hold them whole and registers their scores
+// (NT T / 8 per thread beside the output's NT D / 4), else of 16: 83 against
+// 94 us at 16 sequences of 16384 tokens, D 128.
+template <int D, int GRP, int NT>
+static int attn_tokens(const Kv4AttnArgs& a, const AttnPlan& p, cudaStream_t st) {
+  if constexpr (D < 256 && NT * D <= 256) {
+    if (a.c.P % 32 == 0) return attn_launch<D, GRP, NT, 32>(a, p, st);
+  }
+  return attn_launch<D, GRP, NT, 16>(a, p, st);
+}
+
 template <int D, int GRP>
 static int attn_dispatch(const Kv4AttnArgs& a, const AttnPlan& p, cudaStream_t st) {
   switch (p.nt) {
-    case 1: return attn_launch<D, GRP, 1>(a, p, st);
-    case 2: return attn_launch<D, GRP, 2>(a, p, st);
+    case 1: return attn_tokens<D, GRP, 1>(a, p, st);
+    case 2: return attn_tokens<D, GRP, 2>(a, p, st);
     default:
-      if constexpr (D < 256) return attn_launch<D, GRP, 4>(a, p, st);
+      if constexpr (D < 256) return attn_tokens<D, GRP, 4>(a, p, st);
       return B2K_EUNSUPPORTED;
   }
 }
