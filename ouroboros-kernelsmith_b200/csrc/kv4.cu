@@ -3,20 +3,23 @@
 //
 // One thread holds 8 dimensions of a row (16 bytes on one side, one 32-bit
 // word of nibbles on the other); g / 8 neighbouring lanes reduce their group's
-// minimum and maximum with shuffles.  A block takes 16 tokens and kKvHeads
-// heads of both keys and values, so every thread has four loads in flight and
-// a prefill's writes fill whole micro blocks.  Both are bound by HBM: 2 D Hk
-// values of T on one side, Hk (D + 8 D / g) bytes on the other.
+// minimum and maximum with shuffles.  A block takes 16 tokens, keys and
+// values, and every thread kKvHeads heads, so it has that many loads in flight
+// and a prefill's writes fill whole micro blocks.  Both are bound by HBM: 2 D
+// Hk values of T on one side, Hk (D + 8 D / g) bytes on the other; close to
+// that the instructions per element count too, hence the packed 16-bit
+// arithmetic below.
 #include "kv4.cuh"
 #include "rowio.cuh"
 #include "tma.cuh"
 
 namespace b2k {
 
-constexpr int kKvHeads = 2;
+constexpr int kKvHeads = 4;
 
 struct Kv4IoArgs {
   Kv4 c;
+  FastDiv dP;
   const void *k, *v;      // write: inputs
   void *ko, *vo;          // read: outputs
   const int64_t* slots;
@@ -25,152 +28,220 @@ struct Kv4IoArgs {
   int aligned;
 };
 
-// where a token's slot lies: micro block of head 0 and row within it
-struct Kv4Place {
-  unsigned char* micro;
-  int row;
-  bool in, padding;
+// this thread's row: its token, keys or values, and where the token's slot
+// lies in the pool
+struct Kv4Row {
+  int64_t token;
+  int word, is_v, head;  // first of its heads
+  bool live, in, padding;
+  unsigned char *bits, *par;  // of head 0: the row's words, its parameters
 };
-__device__ __forceinline__ Kv4Place kv4_place(const Kv4IoArgs& a, int64_t slot) {
-  Kv4Place p;
+template <int D> __device__ __forceinline__ Kv4Row kv4_row(const Kv4IoArgs& a) {
+  constexpr int W = D / 8;
+  Kv4Row p;
+  p.word = threadIdx.x % W;
+  p.token = (int64_t)blockIdx.x * 16 + threadIdx.x / W;
+  p.is_v = threadIdx.y;
+  p.head = blockIdx.y * kKvHeads;
+  p.live = p.token < a.T;
+  const int64_t slot = p.live ? a.slots[p.token] : -1;
   p.padding = slot < 0;
   p.in = slot >= 0 && slot < a.c.slots();
   const int64_t s = p.in ? slot : 0;
-  // pools below 2^32 slots (a TB and more) divide in 32 bits
-  const int64_t page = (s >> 32) == 0 ? (int64_t)((uint32_t)s / (uint32_t)a.c.P) : s / a.c.P;
-  const int tok = (int)(s - page * a.c.P);
-  p.micro = a.c.micro(page, 0, tok);
-  p.row = tok & 15;
+  const int64_t page = a.c.slots() < (1ll << 31) ? (int64_t)a.dP.div((int)s) : s / a.c.P;
+  const int tok = (int)(s - page * a.c.P), row = tok & 15, pars = a.c.par_bytes();
+  unsigned char* m = a.c.micro(page, p.head, tok) + p.is_v * (8 * D + 16 * pars);
+  p.bits = m + row * (D / 2) + 4 * (p.is_v ? p.word : kv4_key_word(p.word, D));
+  p.par = m + 8 * D + row * pars + 4 * (p.word / (a.c.g >> 3));
   return p;
 }
 
-// d / s rounded to the nearest whole number, ties to even, and clamped to 0 ..
-// 15, for s > 0 a float16 and r near 1 / s.  The product d r is off by a few
-// 2^-23 of itself, so its nearest whole number n is the quotient's except
-// where that is (almost) halfway.  d - n s is exact there (n s has 15 bits)
-// and tells: beyond s / 2, or equal to it with n odd, the neighbour is meant.
-__device__ __forceinline__ uint32_t kv4_round(float d, float s, float r, float half) {
-  constexpr float kShift = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer
-  const float n = fminf(fmaxf(__fadd_rn(__fadd_rn(d * r, kShift), -kShift), 0.0f), 15.0f);
-  const float rest = fmaf(-n, s, d);
-  uint32_t q = __float_as_uint(n + 8388608.0f) & 15u;
-  if (fabsf(rest) >= half) {
-    // at the ends of the range there is no neighbour
-    const bool move = fabsf(rest) > half || (q & 1u);
-    if (move && rest > 0.0f && q < 15u) ++q;
-    if (move && rest < 0.0f && q > 0u) --q;
+template <typename T> struct Pair16;
+template <> struct Pair16<__half> {
+  using type = __half2;
+  static __device__ __forceinline__ float2 f(__half2 v) { return __half22float2(v); }
+  static __device__ __forceinline__ __half low(__half2 v) { return __low2half(v); }
+  static __device__ __forceinline__ __half high(__half2 v) { return __high2half(v); }
+  static __device__ __forceinline__ __half2 pair(__half a, __half b) { return __halves2half2(a, b); }
+};
+template <> struct Pair16<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+  static __device__ __forceinline__ float2 f(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+  static __device__ __forceinline__ __nv_bfloat16 low(__nv_bfloat162 v) { return __low2bfloat16(v); }
+  static __device__ __forceinline__ __nv_bfloat16 high(__nv_bfloat162 v) { return __high2bfloat16(v); }
+  static __device__ __forceinline__ __nv_bfloat162 pair(__nv_bfloat16 a, __nv_bfloat16 b) {
+    return __halves2bfloat162(a, b);
   }
-  return q;
+};
+
+// n = clamp(rint(d / s), 0, 15) of eight values, as nibbles, for s > 0 a
+// float16.  The product with 1 / s and its rounding give n exactly except
+// where the quotient is (almost) halfway between two integers (the product is
+// off by 2^-22 of itself, 3e-6 at most).  d - n s, whose terms fit fp32 (n s
+// has 15 bits), tells whether any of the eight is that near; then its
+// comparison with s / 2 decides, ties to even.
+__device__ __forceinline__ uint32_t kv4_round8(const float* x, float lo, float s) {
+  constexpr float kShift = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer
+  const float r = rcp_approx(s) * (1.0f / 15.0f), half = 0.5f * s, safe = half * (1.0f - 1e-5f);
+  uint32_t bits = 0;
+  bool near = false;
+#pragma unroll
+  for (int e = 7; e >= 0; --e) {
+    const float d = x[e] - lo;
+    const float t = fmaf(__saturatef(d * r), 15.0f, kShift);
+    near |= fabsf(fmaf(kShift - t, s, d)) >= safe;
+    bits = bits * 16u + __float_as_uint(t);  // 0x4b400000 + n
+  }
+  bits -= 0x4b400000u * 0x11111111u;
+  if (near) {
+    uint32_t fixed = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      uint32_t q = (bits >> (4 * e)) & 15u;
+      const float rest = fmaf(-(float)q, s, x[e] - lo);
+      if (fabsf(rest) > half || (fabsf(rest) == half && (q & 1u)))
+        q = rest > 0.0f ? min(q + 1u, 15u) : q - (q > 0u ? 1u : 0u);
+      fixed |= q << (4 * e);
+    }
+    bits = fixed;
+  }
+  return bits;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(2 * D) kv4_write_kernel(const __grid_constant__ Kv4IoArgs a) {
-  constexpr int W = D / 8;
+// f16(d / 15) with the division rounded to fp32 first.  The product with 1 / 15
+// is within 2 units of the quotient's last place, which float16 drops with 12
+// others: only near a tie of that rounding, or among subnormals, does the
+// division have to be made.
+__device__ __forceinline__ __half kv4_step(float d) {
+  float t = d * (1.0f / 15.0f);
+  const uint32_t low = __float_as_uint(t) & 0x1fffu;
+  if (low - 0xffcu <= 8u || !(t >= 1.2207031e-4f)) t = __fdiv_rn(d, 15.0f);
+  return __float2half_rn(t);
+}
+
+template <typename T, int D, int LANES>
+__global__ void __launch_bounds__(4 * D, 1536 / (4 * D)) kv4_write_kernel(const __grid_constant__ Kv4IoArgs a) {
+  using P = Pair16<T>;
   griddep_launch_dependents();
   griddep_wait();
-  const int word = threadIdx.x % W;
-  const int64_t token = (int64_t)blockIdx.x * 16 + threadIdx.x / W;
-  const bool live = token < a.T;
-  const int64_t slot = live ? a.slots[token] : -1;
-  const int h0 = blockIdx.y * kKvHeads;
-  float x[kKvHeads][2][8];
+  const Kv4Row p = kv4_row<D>(a);
+  const T* src = p.is_v ? static_cast<const T*>(a.v) + p.token * a.ldv + p.head * a.hdv
+                        : static_cast<const T*>(a.k) + p.token * a.ldk + p.head * a.hdk;
+  const int64_t hd = p.is_v ? a.hdv : a.hdk;
+  uint4 raw[kKvHeads];
 #pragma unroll
-  for (int h = 0; h < kKvHeads; ++h)
-#pragma unroll
-    for (int v = 0; v < 2; ++v) {
-      if (live && h0 + h < a.c.Hk) {
-        const T* src = v ? static_cast<const T*>(a.v) + token * a.ldv + (h0 + h) * a.hdv
-                         : static_cast<const T*>(a.k) + token * a.ldk + (h0 + h) * a.hdk;
-        load_vec<T, true>(x[h][v], src, word * 8, D, a.aligned != 0);
+  for (int h = 0; h < kKvHeads; ++h) {
+    raw[h] = zero4();
+    if (p.live && p.head + h < a.c.Hk) {
+      const T* from = src + h * hd + p.word * 8;
+      if (a.aligned) {
+        raw[h] = ld_stream(from);
       } else {
+        float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[h][v][e] = 0.0f;
+        for (int e = 0; e < 8; ++e) x[e] = ld1(from + e);
+        raw[h] = pack<T>(x);
       }
     }
-  const Kv4Place p = kv4_place(a, slot);
-  const int lanes = a.c.g >> 3, rows = 8 * D, half_micro = rows + 16 * a.c.par_bytes();
+  }
   const int64_t head_bytes = (int64_t)(a.c.P >> 4) * a.c.micro_bytes();
 #pragma unroll
-  for (int h = 0; h < kKvHeads; ++h)
+  for (int h = 0; h < kKvHeads; ++h) {
+    // minimum and minus maximum of the group, as a pair
+    const typename P::type* w = reinterpret_cast<const typename P::type*>(&raw[h]);
+    const typename P::type mn = __hmin2_nan(__hmin2_nan(w[0], w[1]), __hmin2_nan(w[2], w[3]));
+    const typename P::type mx = __hmax2_nan(__hmax2_nan(w[0], w[1]), __hmax2_nan(w[2], w[3]));
+    typename P::type ends = P::pair(__hmin_nan(P::low(mn), P::high(mn)),
+                                    __hneg(__hmax_nan(P::low(mx), P::high(mx))));
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {
-      float* y = x[h][v];
-      float lo = INFINITY, hi = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        y[e] = min_nan(max_nan(y[e], -kKv4Limit), kKv4Limit);
-        lo = min_nan(lo, y[e]);
-        hi = max_nan(hi, y[e]);
-      }
-      for (int o = lanes >> 1; o > 0; o >>= 1) {
-        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      }
-      const __half sh = __float2half_rn(__fdiv_rn(hi - lo, 15.0f)), lh = __float2half_rn(lo);
-      const float s = __half2float(sh), l = __half2float(lh);
-      uint32_t bits = 0;
-      if (s > 0.0f) {  // not for a constant group (n = 0), nor a NaN one
-        const float r = __frcp_rn(s), half = 0.5f * s;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) bits |= kv4_round(y[e] - l, s, r, half) << (4 * e);
-      }
-      // a slot outside the pool (negative: padding) is not written
-      if (!p.in || h0 + h >= a.c.Hk) continue;
-      unsigned char* m = p.micro + (h0 + h) * head_bytes + v * half_micro;
-      reinterpret_cast<uint32_t*>(m + p.row * (D / 2))[v ? word : kv4_key_word(word, D)] = bits;
-      if ((word & (lanes - 1)) == 0)
-        reinterpret_cast<__half2*>(m + rows + p.row * a.c.par_bytes())[word / lanes] =
-            __halves2half2(sh, lh);
+    for (int o = LANES >> 1; o > 0; o >>= 1) {
+      uint32_t t = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<uint32_t*>(&ends), o);
+      ends = __hmin2_nan(ends, *reinterpret_cast<typename P::type*>(&t));
     }
+    const float2 f = P::f(ends);
+    float lo = f.x, hi = -f.y, x[8];
+    unpack<T>(raw[h], x);
+    if (!(lo >= -kKv4Limit && hi <= kKv4Limit)) {  // beyond the range, or a NaN
+      lo = min_nan(max_nan(lo, -kKv4Limit), kKv4Limit);
+      hi = min_nan(max_nan(hi, -kKv4Limit), kKv4Limit);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = min_nan(max_nan(x[e], -kKv4Limit), kKv4Limit);
+    }
+    const __half sh = kv4_step(hi - lo), lh = __float2half_rn(lo);
+    const float s = __half2float(sh);
+    // a constant group has n = 0, and so has a NaN one
+    const uint32_t bits = s > 0.0f ? kv4_round8(x, __half2float(lh), s) : 0u;
+    // a slot outside the pool (negative: padding) is not written
+    if (!p.in || p.head + h >= a.c.Hk) continue;
+    *reinterpret_cast<uint32_t*>(p.bits + h * head_bytes) = bits;
+    if ((p.word & (LANES - 1)) == 0)
+      *reinterpret_cast<__half2*>(p.par + h * head_bytes) = __halves2half2(sh, lh);
+  }
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(2 * D) kv4_read_kernel(const __grid_constant__ Kv4IoArgs a) {
-  constexpr int W = D / 8;
+__global__ void __launch_bounds__(4 * D) kv4_read_kernel(const __grid_constant__ Kv4IoArgs a) {
   static_assert(Traits<T>::E == 8, "16-bit outputs");
   griddep_launch_dependents();
   griddep_wait();
-  const int word = threadIdx.x % W;
-  const int64_t token = (int64_t)blockIdx.x * 16 + threadIdx.x / W;
-  if (token >= a.T) return;
-  const Kv4Place p = kv4_place(a, a.slots[token]);
-  const int lanes = a.c.g >> 3, rows = 8 * D, half_micro = rows + 16 * a.c.par_bytes();
+  const Kv4Row p = kv4_row<D>(a);
+  if (!p.live) return;
   const int64_t head_bytes = (int64_t)(a.c.P >> 4) * a.c.micro_bytes();
-  const int h0 = blockIdx.y * kKvHeads;
-  uint32_t bits[kKvHeads][2];
-  __half2 par[kKvHeads][2];
+  uint32_t bits[kKvHeads];
+  __half2 par[kKvHeads];
 #pragma unroll
   for (int h = 0; h < kKvHeads; ++h)
-#pragma unroll
-    for (int v = 0; v < 2; ++v)
-      if (p.in && h0 + h < a.c.Hk) {
-        const unsigned char* m = p.micro + (h0 + h) * head_bytes + v * half_micro;
-        bits[h][v] = __ldcs(reinterpret_cast<const uint32_t*>(m + p.row * (D / 2)) +
-                            (v ? word : kv4_key_word(word, D)));
-        par[h][v] = __ldcs(reinterpret_cast<const __half2*>(m + rows + p.row * a.c.par_bytes()) +
-                           word / lanes);
-      }
-#pragma unroll
-  for (int h = 0; h < kKvHeads; ++h)
-#pragma unroll
-    for (int v = 0; v < 2; ++v) {
-      if (h0 + h >= a.c.Hk) continue;
-      float x[8];
-      if (p.in) {
-        // 2^23 + n as a float; (2^23 + n) s - 2^23 s is n s exactly, fused
-        const float2 f = __half22float2(par[h][v]);
-        const float back = -8388608.0f * f.x;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          x[e] = fmaf(__uint_as_float(((bits[h][v] >> (4 * e)) & 15u) | 0x4b000000u), f.x, back) + f.y;
-      } else {
-        // padding reads zeros; a slot past the pool is an error and reads NaN
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = p.padding ? 0.0f : __int_as_float(0x7fc00000);
-      }
-      T* dst = static_cast<T*>(v ? a.vo : a.ko) + (token * a.c.Hk + h0 + h) * D;
-      store_vec<T>(dst, word * 8, D, true, x);
+    if (p.in && p.head + h < a.c.Hk) {
+      bits[h] = __ldcs(reinterpret_cast<const uint32_t*>(p.bits + h * head_bytes));
+      par[h] = __ldcs(reinterpret_cast<const __half2*>(p.par + h * head_bytes));
     }
+  T* dst = static_cast<T*>(p.is_v ? a.vo : a.ko) + (p.token * a.c.Hk + p.head) * D + p.word * 8;
+#pragma unroll
+  for (int h = 0; h < kKvHeads; ++h) {
+    if (p.head + h >= a.c.Hk) continue;
+    uint4 out;
+    uint32_t* w = &out.x;
+    if (p.in) {
+      // pairs (i, i + 4) as 1024 + n, the integers exactly after that is taken
+      const uint32_t b = bits[h], magic = 0x64006400u;
+      const __half2 m1024 = __float2half2_rn(-1024.0f), m64 = __float2half2_rn(-64.0f),
+                    sixteenth = __float2half2_rn(0.0625f);
+      auto h2 = [](uint32_t v) { return *reinterpret_cast<__half2*>(&v); };
+      __half2 n[4] = {__hadd2(h2((b & 0x000f000fu) | magic), m1024),
+                      __hfma2(h2((b & 0x00f000f0u) | magic), sixteenth, m64),
+                      __hadd2(h2(((b >> 8) & 0x000f000fu) | magic), m1024),
+                      __hfma2(h2(((b >> 8) & 0x00f000f0u) | magic), sixteenth, m64)};
+      if constexpr (std::is_same<T, __half>::value) {
+        // lo + n s with one rounding, then back into order
+        const __half2 s = __low2half2(par[h]), l = __high2half2(par[h]);
+        uint32_t v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const __half2 t = __hfma2(n[e], s, l);
+          v[e] = *reinterpret_cast<const uint32_t*>(&t);
+        }
+        w[0] = __byte_perm(v[0], v[1], 0x5410);
+        w[1] = __byte_perm(v[2], v[3], 0x5410);
+        w[2] = __byte_perm(v[0], v[1], 0x7632);
+        w[3] = __byte_perm(v[2], v[3], 0x7632);
+      } else {
+        const float2 f = __half22float2(par[h]);
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 t = __half22float2(n[e]);
+          x[e] = fmaf(t.x, f.x, f.y);
+          x[e + 4] = fmaf(t.y, f.x, f.y);
+        }
+        out = pack<T>(x);
+      }
+    } else {
+      // padding reads zeros; a slot past the pool is an error and reads NaN
+      const uint32_t fill = p.padding ? 0u : std::is_same<T, __half>::value ? 0x7e007e00u : 0x7fc07fc0u;
+      out = make_uint4(fill, fill, fill, fill);
+    }
+    st_stream(dst + h * D, out);
+  }
 }
 
 }  // namespace b2k
@@ -196,12 +267,17 @@ int kv4_check(const char* what, const void* data, int64_t pages, int64_t Hk, int
   return B2K_OK;
 }
 
+template <typename T, int D> static void kv4_launch_d(const Kv4IoArgs& a, bool write, cudaStream_t st) {
+  const dim3 grid((unsigned)((a.T + 15) / 16), (a.c.Hk + kKvHeads - 1) / kKvHeads), block(2 * D, 2);
+  if (!write) launch_pdl(kv4_read_kernel<T, D>, grid, block, 0, st, a);
+  else if (a.c.g == 32) launch_pdl(kv4_write_kernel<T, D, 4>, grid, block, 0, st, a);
+  else if (a.c.g == 64) launch_pdl(kv4_write_kernel<T, D, 8>, grid, block, 0, st, a);
+  else if constexpr (D >= 128) launch_pdl(kv4_write_kernel<T, D, 16>, grid, block, 0, st, a);
+}
 template <typename T> static void kv4_launch(const Kv4IoArgs& a, bool write, cudaStream_t st) {
-  const dim3 grid((unsigned)((a.T + 15) / 16), (a.c.Hk + kKvHeads - 1) / kKvHeads);
-  auto go = [&](auto w, auto r, int D) { launch_pdl(write ? w : r, grid, dim3(2 * D), 0, st, a); };
-  if (a.c.D == 64) go(kv4_write_kernel<T, 64>, kv4_read_kernel<T, 64>, 64);
-  else if (a.c.D == 128) go(kv4_write_kernel<T, 128>, kv4_read_kernel<T, 128>, 128);
-  else go(kv4_write_kernel<T, 256>, kv4_read_kernel<T, 256>, 256);
+  if (a.c.D == 64) kv4_launch_d<T, 64>(a, write, st);
+  else if (a.c.D == 128) kv4_launch_d<T, 128>(a, write, st);
+  else kv4_launch_d<T, 256>(a, write, st);
 }
 
 }  // namespace b2k
@@ -217,6 +293,7 @@ extern "C" int b2k_kv4_write(const void* k, int64_t ldk, int64_t hdk, const void
   if (T == 0 || pages == 0) return B2K_OK;
   Kv4IoArgs a = {};
   a.c = Kv4{static_cast<unsigned char*>(data), pages, (int)Hk, (int)P, (int)D, (int)group};
+  a.dP = fast_div(P);
   a.k = k; a.v = v; a.slots = slots; a.T = T;
   a.ldk = ldk; a.hdk = hdk; a.ldv = ldv; a.hdv = hdv;
   a.aligned = aligned16(k) && aligned16(v) && ldk % 8 == 0 && hdk % 8 == 0 && ldv % 8 == 0 &&
@@ -239,6 +316,7 @@ extern "C" int b2k_kv4_read(const void* data, int64_t pages, int64_t Hk, int64_t
   Kv4IoArgs a = {};
   a.c = Kv4{static_cast<unsigned char*>(const_cast<void*>(data)), pages, (int)Hk, (int)P, (int)D,
             (int)group};
+  a.dP = fast_div(P);
   a.ko = k; a.vo = v; a.slots = slots; a.T = T;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == B2K_F16) kv4_launch<__half>(a, false, st);

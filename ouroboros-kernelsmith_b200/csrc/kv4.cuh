@@ -28,6 +28,24 @@ namespace b2k {
 
 constexpr float kKv4Limit = 65408.0f;
 
+// n / d for 0 <= n < 2^31 by a multiplication (d is known on the host):
+// with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1,
+// floor(n / d) = (hi32(m n) + n) >> s.
+struct FastDiv {
+  uint32_t d, m, s;
+  __device__ __forceinline__ int div(int n) const {
+    return (int)((__umulhi((uint32_t)n, m) + (uint32_t)n) >> s);
+  }
+};
+inline FastDiv fast_div(int64_t d) {
+  FastDiv f;
+  f.d = (uint32_t)d;
+  f.s = 0;
+  while ((1ll << f.s) < d) ++f.s;
+  f.m = (uint32_t)(((1ull << 32) * ((1ull << f.s) - (uint64_t)d)) / (uint64_t)d + 1);
+  return f;
+}
+
 struct Kv4 {
   unsigned char* data;
   int64_t pages;

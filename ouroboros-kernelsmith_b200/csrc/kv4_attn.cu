@@ -54,23 +54,6 @@ constexpr float kPSlack = 4.0f;   // ... and below 2^(10 + 4) until the maximum 
 constexpr int kAttnLead = 2;      // a segment's fixed costs, in tiles
 constexpr int kAttnLeast = 2;     // tiles of a run beside them
 
-// n / d for 0 <= n < 2^31 by a multiplication (d is known on the host):
-// with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1,
-// floor(n / d) = (hi32(m n) + n) >> s.
-struct FastDiv {
-  uint32_t d, m, s;
-  __device__ __forceinline__ int div(int n) const {
-    return (int)((__umulhi((uint32_t)n, m) + (uint32_t)n) >> s);
-  }
-};
-static FastDiv fast_div(int64_t d) {
-  FastDiv f;
-  f.d = (uint32_t)d;
-  f.s = 0;
-  while ((1ll << f.s) < d) ++f.s;
-  f.m = (uint32_t)(((1ull << 32) * ((1ull << f.s) - (uint64_t)d)) / (uint64_t)d + 1);
-  return f;
-}
 // 64-bit division that takes the short way for what fits 32 bits
 __device__ __forceinline__ int64_t wide_div(int64_t n, int64_t d) {
   if (((n | d) >> 32) == 0) return (uint32_t)n / (uint32_t)d;
