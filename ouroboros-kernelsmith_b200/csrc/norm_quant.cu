@@ -14,7 +14,9 @@
 #include <cuda_fp8.h>
 
 #include "rowio.cuh"
-#include "tma.cuh"
+#include "rowpipe.cuh"
+
+B2K_DEFINE_TIMEOUT_COUNTER()
 
 namespace b2k {
 
@@ -30,9 +32,14 @@ struct NormQuantArgs {
   int aligned;
 };
 
-// NaN-propagating maximum of magnitudes: as unsigned bit patterns a NaN is
-// above infinity, so an integer maximum keeps it (fmaxf would drop it)
-__device__ __forceinline__ uint32_t mag_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// NaN-propagating maximum of magnitudes (fmaxf would drop a NaN).  Between
+// lanes and warps it travels as its bit pattern: as an unsigned integer a NaN
+// is above infinity, so an integer maximum keeps it as well.
+__device__ __forceinline__ float max_mag(float m, float v) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(v)));
+  return r;
+}
 
 // scale and multiplier of a row or group whose largest |y| is `a`
 template <bool I8> __device__ __forceinline__ void quant_scale(float a, float& scale, float& inv) {
@@ -123,16 +130,18 @@ __device__ __forceinline__ void quant_slot(const NormQuantArgs& a, int64_t row, 
                                            float rs, float row_inv, int width) {
   float inv = row_inv;
   if (a.group) {
-    uint32_t m = 0;
+    float mf = 0.0f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) m = max(m, mag_bits(v[e]));
+    for (int e = 0; e < E; ++e) mf = max_mag(mf, v[e]);
+    uint32_t m = __float_as_uint(mf);
     for (int o = width >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     float scale;
     quant_scale<I8>(__uint_as_float(m) * rs, scale, inv);
     if (c < a.N && c % a.group == 0) a.scale[row * a.lds + c / a.group] = scale;
   }
+  const float f = rs * inv;
 #pragma unroll
-  for (int e = 0; e < E; ++e) v[e] = v[e] * rs * inv;
+  for (int e = 0; e < E; ++e) v[e] *= f;
   quant_store<I8, E>(static_cast<uint8_t*>(a.q) + row * a.ldq, c, a.N, a.aligned != 0, v);
 }
 
@@ -155,7 +164,7 @@ __global__ void __launch_bounds__(1024) norm_quant_rows_kernel(NormQuantArgs a) 
   T* hr = static_cast<T*>(a.h) + row * a.ldh;
   float v[V][E];
   float ss = 0.0f;
-  uint32_t mx = 0;
+  float top = 0.0f;
 #pragma unroll
   for (int k = 0; k < V; ++k) {
     const int64_t c = ((int64_t)k * g.G + g.tx) * E;
@@ -176,9 +185,10 @@ __global__ void __launch_bounds__(1024) norm_quant_rows_kernel(NormQuantArgs a) 
     for (int e = 0; e < E; ++e) {
       ss = fmaf(v[k][e], v[k][e], ss);
       v[k][e] *= w[e];
-      mx = max(mx, mag_bits(v[k][e]));
+      top = max_mag(top, v[k][e]);
     }
   }
+  uint32_t mx = __float_as_uint(top);
   group_sum_max(ss, mx, g, red);
   const float rs = rsqrtf(ss / (float)a.N + a.eps);
   float inv = 0.0f;
@@ -211,8 +221,7 @@ __global__ void __launch_bounds__(1024) norm_quant_stream_kernel(NormQuantArgs a
   const T* rr = static_cast<const T*>(a.r) + row * a.ldr;
   const T* wr = static_cast<const T*>(a.w);
   T* hr = static_cast<T*>(a.h) + row * a.ldh;
-  float ss = 0.0f;
-  uint32_t mx = 0;
+  float ss = 0.0f, top = 0.0f;
   auto load = [&](float* v, int64_t c, bool first) {
     load_vec<T, false>(v, xr, c, a.N, al);
     if (a.r) {
@@ -230,9 +239,10 @@ __global__ void __launch_bounds__(1024) norm_quant_stream_kernel(NormQuantArgs a
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       ss = fmaf(v[e], v[e], ss);
-      mx = max(mx, mag_bits(v[e] * w[e]));
+      top = max_mag(top, v[e] * w[e]);
     }
   }
+  uint32_t mx = __float_as_uint(top);
   group_sum_max(ss, mx, g, red);
   const float rs = rsqrtf(ss / (float)a.N + a.eps);
   float inv = 0.0f;
@@ -253,8 +263,149 @@ __global__ void __launch_bounds__(1024) norm_quant_stream_kernel(NormQuantArgs a
   }
 }
 
+// Many aligned rows: persistent blocks on the bulk-copy row pipeline, the
+// weights in registers for all of a block's rows.  One block barrier per row:
+// the warps' partial results alternate between two buffers, and every thread
+// sums them itself.
+template <typename T, bool I8, bool RESID, bool GROUPED, int V, int THREADS>
+__global__ void __launch_bounds__(THREADS) norm_quant_pipe_kernel(const __grid_constant__ NormQuantArgs a,
+                                                              const int S) {
+  constexpr int E = Traits<T>::E, H = E / 2, NIN = RESID ? 2 : 1;
+  extern __shared__ __align__(128) unsigned char dsm[];
+  __shared__ float2 part[2][THREADS / 32];
+  __shared__ volatile int abort_flag;
+  const int tx = threadIdx.x, G = blockDim.x, N = (int)a.N, lane = tx & 31, nw = G >> 5;
+  if (tx == 0) abort_flag = 0;
+  griddep_launch_dependents();
+  const void* srcs[2] = {a.x, a.r};
+  const int64_t lds[2] = {a.ldx, a.ldr};
+  RowPipe<NIN>::prefetch_l2(srcs, lds, (int)sizeof(T), (uint32_t)N * (uint32_t)sizeof(T), a.M, 1);
+  griddep_wait();
+  RowPipe<NIN> pipe;
+  pipe.init(dsm, S, a.M, (uint32_t)N * (uint32_t)sizeof(T), srcs, lds, (int)sizeof(T));
+  uint4 wraw[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const int c = (k * G + tx) * E;
+    wraw[k] = c < N ? ld_keep(static_cast<const T*>(a.w) + c) : zero4();
+  }
+  const int width = a.group / E, gshift = a.group ? __ffs(a.group) - 1 : 0;
+  int64_t n = 0;
+  for (; n < pipe.nrows; ++n) {
+    bool ok;
+    const T* xs = reinterpret_cast<const T*>(pipe.wait_next(ok));
+    if (!ok) {
+      abort_flag = 1;  // every thread leaves after the reduction
+      atomicAdd(&b2k_tu_timeouts, 1u);
+    }
+    const int64_t row = pipe.row_of(n);
+    T* hrow = static_cast<T*>(a.h) + row * a.ldh;
+    float2 v[V][H], ss2 = f2s(0.0f);
+    float top = 0.0f;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const int c = (k * G + tx) * E;
+      if (c < N) {
+        unpack2<T>(*reinterpret_cast<const uint4*>(xs + c), v[k]);
+        if constexpr (RESID) {
+          float2 t[H];
+          unpack2<T>(*reinterpret_cast<const uint4*>(xs + N + c), t);
+#pragma unroll
+          for (int j = 0; j < H; ++j) v[k][j] = add2(v[k][j], t[j]);
+          const uint4 h = pack2<T>(v[k]);
+          st_stream(hrow + c, h);
+          unpack2<T>(h, v[k]);  // the stream as it is stored
+        }
+        float2 w[H];
+        unpack2<T>(wraw[k], w);
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+          ss2 = fma2(v[k][j], v[k][j], ss2);
+          v[k][j] = mul2(v[k][j], w[j]);
+          if constexpr (!GROUPED) top = max_mag(max_mag(top, v[k][j].x), v[k][j].y);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < H; ++j) v[k][j] = f2s(0.0f);
+      }
+    }
+    float ss = ss2.x + ss2.y;
+    uint32_t mx = __float_as_uint(top);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if constexpr (!GROUPED) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    }
+    if (lane == 0) part[n & 1][tx >> 5] = make_float2(ss, __uint_as_float(mx));
+    __syncthreads();  // also: every thread has read the stage
+    if (abort_flag) break;
+    pipe.refill();
+    ss = 0.0f;
+    mx = 0;
+    for (int w = 0; w < nw; ++w) {
+      const float2 t = part[n & 1][w];
+      ss += t.x;
+      if constexpr (!GROUPED) mx = max(mx, __float_as_uint(t.y));
+    }
+    const float rs = rsqrtf(ss / (float)N + a.eps);
+    float inv = 0.0f, scale;
+    if constexpr (!GROUPED) {
+      quant_scale<I8>(__uint_as_float(mx) * rs, scale, inv);
+      if (tx == 0) a.scale[row * a.lds] = scale;
+    }
+    uint8_t* qrow = static_cast<uint8_t*>(a.q) + row * a.ldq;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const int c = (k * G + tx) * E;
+      if constexpr (GROUPED) {
+        float m = 0.0f;
+#pragma unroll
+        for (int j = 0; j < H; ++j) m = max_mag(max_mag(m, v[k][j].x), v[k][j].y);
+        uint32_t mb = __float_as_uint(m);
+        for (int o = width >> 1; o > 0; o >>= 1) mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, o));
+        quant_scale<I8>(__uint_as_float(mb) * rs, scale, inv);
+        if (c < N && (c & (a.group - 1)) == 0) a.scale[row * a.lds + (c >> gshift)] = scale;
+      }
+      const float2 f = f2s(rs * inv);
+#pragma unroll
+      for (int j = 0; j < H; ++j) v[k][j] = mul2(v[k][j], f);
+      quant_store<I8, E>(qrow, c, N, true, reinterpret_cast<const float*>(v[k]));
+    }
+  }
+  pipe.drain(n);
+}
+
+template <typename T, bool I8, bool RESID, bool GROUPED>
+static bool norm_quant_try_pipe(const NormQuantArgs& a, cudaStream_t st) {
+  constexpr int E = Traits<T>::E, NIN = RESID ? 2 : 1;
+  const int64_t nvec = a.N / E, row_bytes = a.N * (int64_t)sizeof(T);
+  if (!a.aligned || (RESID && !a.h) || nvec < 256) return false;
+  // Two vectors per thread up to 256 threads, then four (16381 x 8192 bf16:
+  // 199 us with two, 148 with four; 8192 x 4096 fp16 with its reading back: 61
+  // and 62).  Compiled for 768 threads a kernel has at most 80 registers: more
+  // resident blocks (16000 x 4096 bf16 79 against 84 us, 4000 x 8192 fp32 73
+  // against 81), but four 16-bit vectors spill (16381 x 8192 179 us), so those
+  // are compiled for 512 where that is enough.
+  const int V = nvec <= 512 ? 2 : 4, G = (int)((nvec + 32 * V - 1) / (32 * V)) * 32;
+  if (G > 768) return false;
+  auto kern = V == 2                ? norm_quant_pipe_kernel<T, I8, RESID, GROUPED, 2, 768>
+              : E == 8 && G <= 512 ? norm_quant_pipe_kernel<T, I8, RESID, GROUPED, 4, E == 8 ? 512 : 768>
+                                   : norm_quant_pipe_kernel<T, I8, RESID, GROUPED, 4, 768>;
+  PipeShape ps;
+  if (!choose_pipe_shape(kern, G, NIN * row_bytes, 0, 2, &ps)) return false;
+  int64_t grid = (int64_t)sm_count() * ps.cps;
+  if (a.M < grid) return false;  // a row per block at most: no pipeline to keep
+  launch_pdl(kern, dim3((unsigned)grid), dim3(G), RowPipe<NIN>::smem_bytes(ps.S, row_bytes), st, a, ps.S);
+  return true;
+}
+
 template <typename T, bool I8> static int norm_quant_launch(const NormQuantArgs& a, cudaStream_t st) {
   constexpr int E = Traits<T>::E;
+  const bool piped = a.r ? (a.group ? norm_quant_try_pipe<T, I8, true, true>(a, st)
+                                    : norm_quant_try_pipe<T, I8, true, false>(a, st))
+                         : (a.group ? norm_quant_try_pipe<T, I8, false, true>(a, st)
+                                    : norm_quant_try_pipe<T, I8, false, false>(a, st));
+  if (piped) return check_launch("b2k_norm_quant");
   RowCfg cfg;
   if (!choose_row_cfg(a.N, E, 128, &cfg, 4, 512)) {
     launch_pdl(norm_quant_stream_kernel<T, I8>, dim3((unsigned)a.M), dim3(1024), 0, st, a);
