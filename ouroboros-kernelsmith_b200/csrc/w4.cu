@@ -14,6 +14,8 @@
 #include "rowio.cuh"
 #include "rowpipe.cuh"
 
+B2K_DEFINE_TIMEOUT_COUNTER()
+
 namespace b2k {
 
 struct W4 {
@@ -133,10 +135,11 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const T* w, int64_t ld
 // 2^-25 of its group's maximum; float32 x takes two columns, x' = hi + 2^-11 lo
 // (22 bits).  8-bit x is exact as it is and xs is its scale.
 //
-// Blocks are persistent and hold all of x (their slice of K) in shared memory,
-// prepared once.  KW warps share a row tile, each with every KW-th block of 128
-// columns; loads of the next ones are always in flight, across tiles too.
-constexpr int kW4Smem = 200 << 10;  // shared memory of an SM that x may take
+// Blocks are persistent, one per SM, and hold all of x (their slice of K) in
+// shared memory, prepared once.  KW warps share a row tile, each with a run of
+// its blocks of 128 columns; every warp has its own ring of bulk copies, which
+// runs ahead across tiles.
+constexpr int kW4Stages = 4, kW4Smem = 226 << 10;  // stages at most; of an SM's memory
 
 struct W4Args {
   W4 w;
@@ -151,6 +154,8 @@ struct W4Args {
   int KW;          // warps that share a row tile
   int kslice;      // blocks of 128 columns per grid.z
   int rows;        // rows of x per grid.y
+  int stages;      // of a warp's ring
+  unsigned char* xw;  // x prepared by w4_x_kernel (null: each block prepares its own)
   float* part;     // [grid.z][M][N] partial sums when K is split over blocks
 };
 
@@ -209,22 +214,140 @@ __device__ __forceinline__ void w4_mma(float* c, uint32_t a0, uint32_t a1, uint3
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// row tiles of 16 per warp, and blocks of 128 columns in flight
-__host__ __device__ constexpr int w4_rt(int NT) { return NT == 1 ? 1 : 2; }
-__host__ __device__ constexpr int w4_ring(int NT) { return NT == 1 ? 4 : 2; }
+// the same on zero sums
+__device__ __forceinline__ void w4_mma_first(float* c, uint32_t a0, uint32_t a1, uint32_t a2,
+                                             uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 
-// bytes of x, its groups' sums and scales, and the warps' partial results
+// row tiles of 16 per warp: x's fragments are read once for all of them, which
+// with 16 columns and more would otherwise take more of shared memory's
+// bandwidth than the weights; and blocks of 128 columns in a stage of the ring
+__host__ __device__ constexpr int w4_rt(int NT) { return NT == 1 ? 1 : 2; }
+__host__ __device__ constexpr int w4_sbk(int NT) { return 2 / w4_rt(NT); }
+// stage: 2 KB of weights, then the scales and the zeros of their groups
+__host__ __device__ constexpr int w4_stage(int gs) { return 2048 + 128 * gs; }
+// bytes of x, and of its groups' sums and scales, for kslice blocks of columns;
+// and of both for all of K in the workspace
 __host__ __device__ inline int64_t w4_x_bytes(int64_t kslice, int cols) { return kslice * 256 * cols; }
 __host__ __device__ inline int64_t w4_g_bytes(int64_t kslice, int gs, int NT) {
   return kslice * gs * 64 * NT;
 }
-__host__ __device__ constexpr int w4_red_bytes(int NT) { return w4_rt(NT) * 16 * 8 * NT * 4; }
+__host__ __device__ inline int64_t w4_image_bytes(int64_t KT, int cols, int gs, int NT) {
+  return w4_x_bytes(KT, cols) + w4_g_bytes(KT, gs, NT);
+}
+
+// Eight columns of one row of x (column 128 kb0 + 8 v8) into the form that the
+// products read, by all lanes of a warp (`live`: this lane has any):
+//   xo  [32 columns][C][quarter] of 16 bytes: columns (0,4) (2,6) and, / 16,
+//       (1,5) (3,7) of the quarter's eight, the order of the unpacked words
+//   go  [group][pitch] of (sum, scale)
+template <int GS>
+__device__ __forceinline__ void w4_stage_eight(const W4Args& a, int64_t row, int64_t kb0, int v8,
+                                               bool live, int m, int C, unsigned char* xo,
+                                               float2* go, int pitch) {
+  constexpr int G = 128 / GS;
+  const bool f32 = a.xtype == B2K_F32;
+  const int64_t k = kb0 * 128 + (int64_t)v8 * 8;
+  float v[8];
+  if (live) {
+    w4_x8(a, row, k, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+  }
+  float f = 1.0f, xs;
+  if (a.xs) {
+    const int64_t g = a.xgroup ? k / a.xgroup : 0;
+    xs = live && k < a.w.K ? a.xs[row * a.ldxs + g] * 16384.0f : 0.0f;
+    // a group of 8-bit values that are not finite, or of such a scale, is NaN
+    bool odd = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) odd |= !isfinite(v[e]);
+    if (odd || !isfinite(xs)) xs = __int_as_float(0x7fc00000);
+#pragma unroll
+    for (int o = 1; o < G / 8; o <<= 1) {
+      const float t = __shfl_xor_sync(0xffffffffu, xs, o);
+      if (t != t || k >= a.w.K) xs = t;
+    }
+  } else {
+    uint32_t top = 0;  // magnitudes as integers: a NaN stays on top
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 1; o < G / 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int ex = (int)(top >> 23);
+    if (ex == 255) {
+      xs = __int_as_float(0x7fc00000);
+    } else {
+      const int fb = min(268 - ex, 254);
+      f = __uint_as_float((uint32_t)fb << 23);
+      xs = __uint_as_float((uint32_t)(268 - fb) << 23);
+    }
+  }
+  for (int part = 0; part < (f32 ? 2 : 1); ++part) {
+    const int col = f32 ? 2 * m + part : m;
+    __half h[8], h16[8];
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float t = part == 0 ? v[e] * f : v[e];
+      h[e] = __float2half_rn(t);
+      const float back = __half2float(h[e]);
+      sum += back;
+      h16[e] = __float2half_rn(back * 0.0625f);
+      v[e] = (t - back) * 2048.0f;
+    }
+#pragma unroll
+    for (int o = 1; o < G / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (live) {
+      *reinterpret_cast<uint4*>(xo + ((int64_t)(v8 >> 2) * C + col) * 64 + (v8 & 3) * 16) =
+          make_uint4(h2_bits(h[0], h[4]), h2_bits(h[2], h[6]), h2_bits(h16[1], h16[5]),
+                     h2_bits(h16[3], h16[7]));
+      // the sum in units of the products, 2^-24
+      if (v8 % (G / 8) == 0)
+        go[(int64_t)(v8 / (G / 8)) * pitch + col] = f2(sum * 5.9604644775390625e-8f, xs);
+    }
+  }
+}
+
+// The whole of x, once, in the form of the blocks' shared memory: for every
+// grid.y of the product its rows' image and their groups (zeros for columns
+// past the rows).  A warp takes 32 eights of a row.
+template <int GS>
+__global__ void __launch_bounds__(256) w4_x_kernel(const __grid_constant__ W4Args a, int nt) {
+  griddep_wait();
+  // Only now: the product starts on its weights before it waits for this grid,
+  // and what came before this grid may have written them.
+  griddep_launch_dependents();
+  const int64_t KT = a.w.ktiles(), per_row = KT * 16;
+  const int per = a.xtype == B2K_F32 ? 2 : 1, cols = a.rows * per;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t y = blockIdx.y, m0 = y * a.rows;
+  const int rows = (int)min((int64_t)a.rows, a.M - m0);
+  const bool live = i < rows * per_row;
+  const int m = live ? (int)(i / per_row) : 0;
+  const int v8 = live ? (int)(i - m * per_row) : 0;
+  unsigned char* xo = a.xw + y * w4_image_bytes(KT, cols, GS, nt);
+  float2* go = reinterpret_cast<float2*>(xo + KT * 256 * cols);
+  w4_stage_eight<GS>(a, m0 + m, 0, v8, live, m, rows * per, xo, go, 8 * nt);
+  if (live && m == 0 && v8 % (16 / GS) == 0)
+    for (int col = rows * per; col < 8 * nt; ++col)
+      go[(int64_t)(v8 / (16 / GS)) * 8 * nt + col] = f2(0.0f, 0.0f);
+}
 
 // GS = groups per 128 columns, 8 NT = columns (rows of x; two each for float32)
 template <int NT, int GS> __global__ void __launch_bounds__(512, 1) w4_kernel(
     const __grid_constant__ W4Args a) {
-  constexpr int RT = w4_rt(NT), UK = w4_ring(NT), G = 128 / GS;
+  constexpr int RT = w4_rt(NT), SBK = w4_sbk(NT), G = 128 / GS, STAGE = w4_stage(GS);
+  const int S = a.stages;
   extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ uint64_t full[16][kW4Stages], xbar;
+  __shared__ int red_at[16];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
   const int nwarps = blockDim.x >> 5;
   const int64_t KT = a.w.ktiles(), tiles = a.w.ntiles();
@@ -232,178 +355,141 @@ template <int NT, int GS> __global__ void __launch_bounds__(512, 1) w4_kernel(
   const int kn = (int)min((int64_t)a.kslice, KT - kb0);  // blocks of this slice
   const int64_t m0 = (int64_t)blockIdx.y * a.rows;
   const int rows = (int)min((int64_t)a.rows, a.M - m0);
-  const bool f32 = a.xtype == B2K_F32;
+  const bool f32 = a.xtype == B2K_F32, zeros = a.w.zeros != nullptr;
   const int C = f32 ? 2 * rows : rows;
-  unsigned char* xsm = smem;
-  float2* gsm = reinterpret_cast<float2*>(smem + w4_x_bytes(a.kslice, f32 ? 2 * a.rows : a.rows));
-  float* red = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(gsm) +
-                                        w4_g_bytes(a.kslice, GS, NT));
+  unsigned char* ring = smem + warp * (S * STAGE);
+  unsigned char* xsm = smem + nwarps * (S * STAGE);
+  float2* gsm = reinterpret_cast<float2*>(xsm + w4_x_bytes(a.kslice, f32 ? 2 * a.rows : a.rows));
 
   // ---- this warp's stream of weights ---------------------------------------
   const int KW = a.KW, kw = warp % KW, grp = warp / KW, groups = nwarps / KW;
+  const int chunk = (kn + KW - 1) / KW;
+  const int k0 = min(kn, kw * chunk), k1 = min(kn, k0 + chunk);  // its blocks
   const int64_t items = (tiles + RT - 1) / RT, step = (int64_t)gridDim.x * groups;
   const int64_t first = (int64_t)blockIdx.x * groups + grp;
-  uint4 wa[UK][RT], wb[UK][RT];
-  uint32_t ws[UK][RT], wz[UK][RT];
   int64_t pit = first;  // next to load
-  int pk = kw;
-  auto load = [&](int u) {
-    if (pit < items && pk < kn) {
+  int pk = k0, get_stage = 0, use_stage = 0;
+  uint32_t use_phase = 0, issued = 0, used = 0;
+  bool dead = false;  // a wait ran out
+  auto issue = [&]() {
+    const int n = min(SBK, k1 - pk);
+    if (lane == 0) {
+      uint64_t* bar = &full[warp][get_stage];
+      unsigned char* dst = ring + get_stage * STAGE;
+      const uint32_t wb = n * 1024, sb = n * GS * 32;
+      fence_proxy_async();
+      mbar_arrive_expect_tx(bar, RT * (wb + (zeros ? 2 : 1) * sb));
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        const int64_t tile = min(pit * RT + t, tiles - 1);
-        const int64_t at = tile * KT + kb0 + pk;
-        const uint4* p = reinterpret_cast<const uint4*>(a.w.tiles) + at * 64 + lane;
-        wa[u][t] = __ldcs(p);
-        wb[u][t] = __ldcs(p + 32);
-        const int64_t si = (at * GS + c % GS) * 16 + r;
-        const uint16_t* sp = static_cast<const uint16_t*>(a.w.scales) + si;
-        ws[u][t] = (uint32_t)__ldcs(sp) | ((uint32_t)__ldcs(sp + 8) << 16);
-        if (a.w.zeros) {
-          const uint16_t* zp = static_cast<const uint16_t*>(a.w.zeros) + si;
-          wz[u][t] = (uint32_t)__ldcs(zp) | ((uint32_t)__ldcs(zp + 8) << 16);
-        }
+        const int64_t at = min(pit * RT + t, tiles - 1) * KT + kb0 + pk;
+        bulk_g2s(dst + t * SBK * 1024, a.w.tiles + at * 1024, wb, bar);
+        bulk_g2s(dst + 2048 + t * SBK * GS * 32,
+                 static_cast<const unsigned char*>(a.w.scales) + at * GS * 32, sb, bar);
+        if (zeros)
+          bulk_g2s(dst + 2048 + (2 * GS + t * SBK * GS) * 32,
+                   static_cast<const unsigned char*>(a.w.zeros) + at * GS * 32, sb, bar);
       }
-      pk += KW;
-      if (pk >= kn) {
-        pk = kw;
-        pit += step;
-      }
+    }
+    if (++get_stage == S) get_stage = 0;
+    ++issued;
+    pk += n;
+    if (pk >= k1) {
+      pk = k0;
+      pit += step;
     }
   };
   griddep_launch_dependents();
-  griddep_wait();
-  if (kw < kn) {
-#pragma unroll
-    for (int u = 0; u < UK; ++u) load(u);
-  }
+  if (lane < S) mbar_init(&full[warp][lane], 1);
+  fence_barrier_init();
+  __syncwarp();
+  // With x prepared by the kernel before, the weights need not wait for it.
+  if (!a.xw) griddep_wait();
+  if (k0 < k1)
+    for (int s = 0; s < S && pit < items; ++s) issue();
+  if (a.xw) griddep_wait();
 
   // ---- x into shared memory -------------------------------------------------
-  // [32 columns][C][quarter c] of 16 bytes: columns (0,4) (2,6) and, / 16,
-  // (1,5) (3,7) of the quarter's eight, the order of the unpacked words
-  {
-    const int per_row = kn * 16;  // eights of columns
-    const int total = rows * per_row;
-    for (int i = tid; i < kn * GS * 8 * NT; i += blockDim.x) gsm[i] = f2(0.0f, 0.0f);
+  for (int i = tid; i < kn * GS * 8 * NT; i += blockDim.x) gsm[i] = f2(0.0f, 0.0f);
+  if (a.xw) {  // prepared by w4_x_kernel
+    if (tid == 0) {
+      mbar_init(&xbar, 1);
+      fence_barrier_init();
+    }
     __syncthreads();
+    if (tid == 0) {
+      const unsigned char* xw = a.xw + (int64_t)blockIdx.y * w4_image_bytes(KT, f32 ? 2 * a.rows : a.rows, GS, NT);
+      const uint32_t xb = kn * 256 * C, gb = kn * GS * 64 * NT;
+      fence_proxy_async();
+      mbar_arrive_expect_tx(&xbar, xb + gb);
+      for (uint32_t o = 0; o < xb; o += 32768)
+        bulk_g2s(xsm + o, xw + kb0 * 256 * C + o, min(xb - o, 32768u), &xbar);
+      bulk_g2s(gsm, xw + KT * 256 * (f32 ? 2 * a.rows : a.rows) + kb0 * GS * 64 * NT, gb, &xbar);
+    }
+    if (!mbar_wait(&xbar, 0)) {
+      dead = true;
+      if (lane == 0) atomicAdd(&b2k_tu_timeouts, 1u);
+    }
+  } else {
+    __syncthreads();
+    const int per_row = kn * 16, total = rows * per_row;  // eights of columns
     for (int base = warp * 32; base < total; base += blockDim.x) {
-      const int i = base + lane;
-      const bool live = i < total;
-      const int m = live ? i / per_row : 0, v8 = live ? i - m * per_row : 0;
-      const int64_t k = kb0 * 128 + v8 * 8;
-      float v[8];
-      if (live) {
-        w4_x8(a, m0 + m, k, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-      }
-      float f = 1.0f, xs;
-      if (a.xs) {
-        const int64_t g = a.xgroup ? k / a.xgroup : 0;
-        xs = live && k < a.w.K ? a.xs[(m0 + m) * a.ldxs + g] * 16384.0f : 0.0f;
-        // a group of 8-bit values that are not finite, or of such a scale, is NaN
-        bool odd = false;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) odd |= !isfinite(v[e]);
-        if (odd) xs = __int_as_float(0x7fc00000);
-#pragma unroll
-        for (int o = 1; o < G / 8; o <<= 1) {
-          const float t = __shfl_xor_sync(0xffffffffu, xs, o);
-          if (t != t || k >= a.w.K) xs = t;
-        }
-      } else {
-        uint32_t top = 0;  // magnitudes as integers: a NaN stays on top
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
-#pragma unroll
-        for (int o = 1; o < G / 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const int ex = (int)(top >> 23);
-        if (ex == 255) {
-          xs = __int_as_float(0x7fc00000);
-        } else {
-          const int fb = min(268 - ex, 254);
-          f = __uint_as_float((uint32_t)fb << 23);
-          xs = __uint_as_float((uint32_t)(268 - fb) << 23);
-        }
-      }
-      for (int part = 0; part < (f32 ? 2 : 1); ++part) {
-        const int col = f32 ? 2 * m + part : m;
-        __half h[8], h16[8];
-        float sum = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float t = part == 0 ? v[e] * f : v[e];
-          h[e] = __float2half_rn(t);
-          const float back = __half2float(h[e]);
-          sum += back;
-          h16[e] = __float2half_rn(back * 0.0625f);
-          v[e] = (t - back) * 2048.0f;
-        }
-#pragma unroll
-        for (int o = 1; o < G / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (live) {
-          *reinterpret_cast<uint4*>(xsm + ((int64_t)(v8 >> 2) * C + col) * 64 + (v8 & 3) * 16) =
-              make_uint4(h2_bits(h[0], h[4]), h2_bits(h[2], h[6]), h2_bits(h16[1], h16[5]),
-                         h2_bits(h16[3], h16[7]));
-          // the sum in units of the products, 2^-24
-          if (v8 % (G / 8) == 0)
-            gsm[(v8 / (G / 8)) * 8 * NT + col] = f2(sum * 5.9604644775390625e-8f, xs);
-        }
-      }
+      const int i = base + lane, m = min(i, total - 1) / per_row;
+      w4_stage_eight<GS>(a, m0 + m, kb0, i - m * per_row, i < total, m, C, xsm, gsm, 8 * NT);
     }
     __syncthreads();
   }
 
   // ---- the group's warps add up a tile; its rows are columns of y ------------
-  auto join = [&](int64_t it, float (&y)[RT][NT][4]) {
-    constexpr int PER = RT * 16 * 8 * NT;
-    if (KW > 1) named_bar_sync(1 + grp, 32 * KW);  // the last tile's sums are read
-    float* mine = red + (int64_t)warp * PER;       // [column][RT * 16 rows]
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          mine[(nt * 8 + 2 * c + (e & 1)) * RT * 16 + t * 16 + r + 8 * (e >> 1)] = y[t][nt][e];
+  // Their parts lie in the stages that they have just read.
+  const int odd = r & 1, row_a = 2 * r + odd, row_b = 2 * r + 1 - odd;  // rows r, r + 8 of the products
+  auto sync_group = [&]() {
     if (KW > 1) named_bar_sync(1 + grp, 32 * KW);
     else __syncwarp();
-    const float* from = red + (int64_t)(grp * KW) * PER;
-    for (int i = kw * 32 + lane; i < rows * RT * 16; i += 32 * KW) {
-      const int m = i / (RT * 16), n16 = i - m * (RT * 16);
-      const int64_t n = it * (RT * 16) + n16;
-      if (n >= a.w.N) continue;
-      float v = 0.0f;
-      if (f32) {
-        float lo = 0.0f;
-        for (int w = 0; w < KW; ++w) {
-          v += from[w * PER + (2 * m) * RT * 16 + n16];
-          lo += from[w * PER + (2 * m + 1) * RT * 16 + n16];
-        }
-        v = fmaf(lo, 0.00048828125f, v);
-      } else {
-        for (int w = 0; w < KW; ++w) v += from[w * PER + i];
-      }
-      if (a.part) {
-        a.part[((int64_t)blockIdx.z * a.M + m0 + m) * a.w.N + n] = v;
-        continue;
-      }
-      const int64_t at = (m0 + m) * a.ldy + n;
-      if (a.ytype == B2K_F32) static_cast<float*>(a.y)[at] = v;
-      else if (a.ytype == B2K_F16) static_cast<__half*>(a.y)[at] = from_f<__half>(v);
-      else static_cast<__nv_bfloat16*>(a.y)[at] = from_f<__nv_bfloat16>(v);
-    }
-    if (KW == 1) __syncwarp();
+  };
+  auto join = [&](int64_t it, int stage, float (&y)[RT][NT][4]) {
+    if (lane == 0) red_at[warp] = warp * (S * STAGE) + stage * STAGE;
+    float* mine = reinterpret_cast<float*>(ring + stage * STAGE);  // [column][16 rows]
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
+    for (int t = 0; t < RT; ++t) {
+      __syncwarp();  // this warp has read the stage
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[t][nt][e] = 0.0f;
+        for (int e = 0; e < 4; ++e) {
+          mine[(nt * 8 + 2 * c + (e & 1)) * 16 + (e >> 1 ? row_b : row_a)] = y[t][nt][e];
+          y[t][nt][e] = 0.0f;
+        }
+      sync_group();
+      for (int i = kw * 32 + lane; i < rows * 16; i += 32 * KW) {
+        const int m = i >> 4, n16 = i & 15;
+        const int64_t n = (it * RT + t) * 16 + n16;
+        if (n >= a.w.N) continue;
+        float v = 0.0f;
+        if (f32) {
+          float lo = 0.0f;
+          for (int w = 0; w < KW; ++w) {
+            const float* from = reinterpret_cast<const float*>(smem + red_at[grp * KW + w]);
+            v += from[2 * m * 16 + n16];
+            lo += from[(2 * m + 1) * 16 + n16];
+          }
+          v = fmaf(lo, 0.00048828125f, v);
+        } else {
+          for (int w = 0; w < KW; ++w)
+            v += reinterpret_cast<const float*>(smem + red_at[grp * KW + w])[i];
+        }
+        if (a.part) {
+          a.part[((int64_t)blockIdx.z * a.M + m0 + m) * a.w.N + n] = v;
+          continue;
+        }
+        const int64_t at = (m0 + m) * a.ldy + n;
+        if (a.ytype == B2K_F32) static_cast<float*>(a.y)[at] = v;
+        else if (a.ytype == B2K_F16) static_cast<__half*>(a.y)[at] = from_f<__half>(v);
+        else static_cast<__nv_bfloat16*>(a.y)[at] = from_f<__nv_bfloat16>(v);
+      }
+      sync_group();
+    }
   };
 
-  // ---- tiles, as one stream of blocks whose ring slots are taken in turn ----
   float y[RT][NT][4];
 #pragma unroll
   for (int t = 0; t < RT; ++t)
@@ -411,90 +497,101 @@ template <int NT, int GS> __global__ void __launch_bounds__(512, 1) w4_kernel(
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[t][nt][e] = 0.0f;
-  int k = kw;
-  for (int64_t it = first; it < items;) {
+  const uint32_t swap = odd ? 0x1032u : 0x3210u;
+
+  for (int64_t it = first; it < items; it += step) {
+    int stage = 0;
+    for (int k = k0; k < k1; k += SBK) {
+      stage = use_stage;
+      if (!dead && !mbar_wait(&full[warp][stage], use_phase)) {
+        // stay in step with the group's barriers; the results are lost
+        dead = true;
+        if (lane == 0) atomicAdd(&b2k_tu_timeouts, 1u);
+      }
+      ++used;
+      if (++use_stage == S) {
+        use_stage = 0;
+        use_phase ^= 1;
+      }
+      const unsigned char* st = ring + stage * STAGE;
 #pragma unroll
-    for (int u = 0; u < UK; ++u) {
-      if (it < items) {
-        if (k < kn) {
-          float acc[RT][NT][4];
+      for (int i = 0; i < SBK; ++i) {
+        if (SBK > 1 && k + i >= k1) break;
+        uint4 wa[RT], wb[RT];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (j * 32 % G == 0) {
+        for (int t = 0; t < RT; ++t) {
+          const unsigned char* p = st + (t * SBK + i) * 1024 + c * 16;
+          wa[t] = *reinterpret_cast<const uint4*>(p + row_a * 64);
+          wb[t] = *reinterpret_cast<const uint4*>(p + row_b * 64);
+        }
+        float acc[RT][NT][4];
 #pragma unroll
-              for (int t = 0; t < RT; ++t)
+        for (int j = 0; j < 4; ++j) {
+          const unsigned char* xp = xsm + (int64_t)(4 * (k + i) + j) * C * 64 + r * 64 + c * 16;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt) {
+            uint4 b = zero4();
+            if (nt * 8 + r < C) b = *reinterpret_cast<const uint4*>(xp + nt * 512);
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) acc[t][nt][e] = 0.0f;
-            }
-            const unsigned char* xp = xsm + (int64_t)(4 * k + j) * C * 64 + r * 64 + c * 16;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              uint4 b = zero4();
-              if (nt * 8 + r < C) b = *reinterpret_cast<const uint4*>(xp + nt * 512);
-#pragma unroll
-              for (int t = 0; t < RT; ++t) {
-                const uint32_t w0 = j == 0 ? wa[u][t].x : j == 1 ? wa[u][t].y : j == 2 ? wa[u][t].z : wa[u][t].w;
-                const uint32_t w1 = j == 0 ? wb[u][t].x : j == 1 ? wb[u][t].y : j == 2 ? wb[u][t].z : wb[u][t].w;
-                const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
+            for (int t = 0; t < RT; ++t) {
+              const uint32_t w0 = j == 0 ? wa[t].x : j == 1 ? wa[t].y : j == 2 ? wa[t].z : wa[t].w;
+              const uint32_t w1 = j == 0 ? wb[t].x : j == 1 ? wb[t].y : j == 2 ? wb[t].z : wb[t].w;
+              const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
+              if (j * 32 % G == 0)
+                w4_mma_first(acc[t][nt], w0 & 0x000f000fu, w1 & 0x000f000fu, v0 & 0x000f000fu,
+                             v1 & 0x000f000fu, b.x, b.y);
+              else
                 w4_mma(acc[t][nt], w0 & 0x000f000fu, w1 & 0x000f000fu, v0 & 0x000f000fu,
                        v1 & 0x000f000fu, b.x, b.y);
-                w4_mma(acc[t][nt], w0 & 0x00f000f0u, w1 & 0x00f000f0u, v0 & 0x00f000f0u,
-                       v1 & 0x00f000f0u, b.z, b.w);
-              }
+              w4_mma(acc[t][nt], w0 & 0x00f000f0u, w1 & 0x00f000f0u, v0 & 0x00f000f0u,
+                     v1 & 0x00f000f0u, b.z, b.w);
             }
-            if ((j + 1) * 32 % G == 0) {
-              const int gi = j * 32 / G;
-              const float4* gp = reinterpret_cast<const float4*>(gsm + (k * GS + gi) * 8 * NT + 2 * c);
-              float4 g4[NT];  // (sum, scale) of columns 2c, 2c + 1
+          }
+          if ((j + 1) * 32 % G == 0) {
+            const int gi = j * 32 / G;
+            const float4* gp = reinterpret_cast<const float4*>(gsm + ((k + i) * GS + gi) * 8 * NT + 2 * c);
+            float4 g4[NT];  // (sum, scale) of columns 2c, 2c + 1
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) g4[nt] = gp[nt * 4];
+            for (int nt = 0; nt < NT; ++nt) g4[nt] = gp[nt * 4];
 #pragma unroll
-              for (int t = 0; t < RT; ++t) {
-                const int src = (lane & ~3) | gi;
-                const uint32_t sb = GS == 1 ? ws[u][t] : __shfl_sync(0xffffffffu, ws[u][t], src);
-                float s0, s1, z0 = 8.0f, z1 = 8.0f;
-                if (a.stype == B2K_F16) {
-                  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&sb));
-                  s0 = f.x; s1 = f.y;
-                } else {
-                  s0 = __uint_as_float(sb << 16); s1 = __uint_as_float(sb & 0xffff0000u);
-                }
-                if (a.w.zeros) {
-                  const uint32_t zb = GS == 1 ? wz[u][t] : __shfl_sync(0xffffffffu, wz[u][t], src);
-                  if (a.stype == B2K_F16) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&zb));
-                    z0 = f.x; z1 = f.y;
-                  } else {
-                    z0 = __uint_as_float(zb << 16); z1 = __uint_as_float(zb & 0xffff0000u);
-                  }
-                }
-                s0 *= 1024.0f;  // 2^24 of the integers' unit, 2^-14 of x's
-                s1 *= 1024.0f;
+            for (int t = 0; t < RT; ++t) {
+              // rows 2r, 2r + 1 of the tile
+              const uint32_t* sp = reinterpret_cast<const uint32_t*>(
+                  st + 2048 + ((t * SBK + i) * GS + gi) * 32) + r;
+              auto two = [&](uint32_t bits) {
+                bits = __byte_perm(bits, 0, swap);
+                if (a.stype == B2K_F16) return __half22float2(*reinterpret_cast<const __half2*>(&bits));
+                return f2(__uint_as_float(bits << 16), __uint_as_float(bits & 0xffff0000u));
+              };
+              const float2 z = zeros ? two(sp[2 * GS * 8]) : f2s(8.0f);
+              // 2^10: 2^24 of the integers' unit, 2^-14 of x's
+              const float2 s = mul2(two(*sp), f2s(1024.0f));
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                  float* q = acc[t][nt];
-                  const float4 g = g4[nt];
-                  y[t][nt][0] = fmaf(fmaf(-z0, g.x, q[0]) * s0, g.y, y[t][nt][0]);
-                  y[t][nt][1] = fmaf(fmaf(-z0, g.z, q[1]) * s0, g.w, y[t][nt][1]);
-                  y[t][nt][2] = fmaf(fmaf(-z1, g.x, q[2]) * s1, g.y, y[t][nt][2]);
-                  y[t][nt][3] = fmaf(fmaf(-z1, g.z, q[3]) * s1, g.w, y[t][nt][3]);
-                }
+              for (int nt = 0; nt < NT; ++nt) {
+                const float* q = acc[t][nt];
+                const float4 g = g4[nt];
+                y[t][nt][0] = fmaf(fmaf(-z.x, g.x, q[0]) * s.x, g.y, y[t][nt][0]);
+                y[t][nt][1] = fmaf(fmaf(-z.x, g.z, q[1]) * s.x, g.w, y[t][nt][1]);
+                y[t][nt][2] = fmaf(fmaf(-z.y, g.x, q[2]) * s.y, g.y, y[t][nt][2]);
+                y[t][nt][3] = fmaf(fmaf(-z.y, g.z, q[3]) * s.y, g.w, y[t][nt][3]);
               }
             }
           }
-          load(u);
-        }
-        k += KW;
-        if (k >= kn) {
-          join(it, y);
-          k = kw;
-          it += step;
         }
       }
+      if (k + SBK < k1) {  // the last stage of a tile is needed for the join
+        __syncwarp();
+        if (!dead && pit < items) issue();
+      }
     }
+    join(it, stage, y);
+    if (k0 < k1 && !dead && pit < items) issue();
   }
+  if (dead)  // nothing may land after the block has gone
+    for (; used <= issued && used > 0; ++used) {
+      const uint32_t t = used - 1;  // the tile that was given up, and those after it
+      if (t < issued) mbar_wait(&full[warp][t % S], (t / S) & 1);
+    }
 }
 
 // y = the sum of K's slices, in order
@@ -511,45 +608,48 @@ template <typename T> __global__ void __launch_bounds__(256) w4_sum_kernel(const
   }
 }
 
-// How a product is split.  Blocks are of 8 warps, two per SM, while x fits half
-// an SM's shared memory, else of 16; K is split over blocks only when x does
-// not fit at all.  KW is the number of warps per tile that leaves the longest
-// warp the least to do, counting a tile's join as two blocks of 128 columns.
+// How a product is split.  One block of 16 warps per SM, their rings as deep as
+// shared memory allows beside x (2 to kW4Stages stages); K is split over blocks
+// where x does not fit beside two.  x is prepared once by a kernel of its own
+// where every block's own preparation would take it more than kW4Own eights of
+// columns per thread.  KW is the number of warps per tile that leaves the
+// longest warp the least to do, counting a tile's join as two blocks of 128
+// columns.
+constexpr int kW4Own = 4;
 struct W4Plan {
-  int nt, rows, warps, cps, kslice, slices, kw, grid_x, grid_y;
-  int64_t smem, bytes;
+  int nt, rows, warps, stages, kslice, slices, kw, grid_x, grid_y;
+  bool prepare;
+  int64_t smem, image, bytes;
 };
 
 static W4Plan w4_plan(int64_t M, int64_t N, int64_t K, int group, bool f32) {
   W4Plan p;
-  const int per = f32 ? 2 : 1;
+  const int per = f32 ? 2 : 1, gs = 128 / group;
   const int64_t cols = M * per, KT = (K + 127) / 128, tiles = (N + 15) / 16;
   p.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
   p.rows = (int)(M < 8 * p.nt / per ? M : 8 * p.nt / per);
   p.grid_y = (int)((M + p.rows - 1) / p.rows);
-  const int gs = 128 / group;
-  auto need = [&](int64_t kslice, int warps) {
+  p.warps = 16;
+  auto need = [&](int64_t kslice, int stages) {
     return w4_x_bytes(kslice, p.rows * per) + w4_g_bytes(kslice, gs, p.nt) +
-           (int64_t)warps * w4_red_bytes(p.nt);
+           (int64_t)p.warps * stages * w4_stage(gs);
   };
   p.slices = 1;
   p.kslice = (int)(KT > 0 ? KT : 1);
-  p.warps = 8;
-  p.cps = 2;
-  if (need(p.kslice, 8) > kW4Smem / 2) {
-    p.warps = 16;
-    p.cps = 1;
-    while (need(p.kslice, 16) > kW4Smem) {
-      ++p.slices;
-      p.kslice = (int)((KT + p.slices - 1) / p.slices);
-    }
-    p.slices = (int)((KT + p.kslice - 1) / p.kslice);
+  while (need(p.kslice, 2) > kW4Smem) {
+    ++p.slices;
+    p.kslice = (int)((KT + p.slices - 1) / p.slices);
   }
-  p.smem = need(p.kslice, p.warps);
+  p.slices = KT > 0 ? (int)((KT + p.kslice - 1) / p.kslice) : 1;
+  p.stages = kW4Stages;
+  while (need(p.kslice, p.stages) > kW4Smem) --p.stages;
+  p.prepare = (int64_t)p.rows * p.kslice * 16 > kW4Own * 32 * p.warps;
+  p.smem = need(p.kslice, p.stages);
   const int64_t items = (tiles + w4_rt(p.nt) - 1) / w4_rt(p.nt);
-  int64_t slots = (int64_t)sm_count() * p.cps / (p.slices * p.grid_y);
+  int64_t slots = (int64_t)sm_count() / (p.slices * p.grid_y);
   if (slots < 1) slots = 1;
   int64_t best = -1;
+  p.kw = 1;
   for (int kw = 1; kw <= p.warps; kw <<= 1) {
     const int64_t rounds = (items * kw + slots * p.warps - 1) / (slots * p.warps);
     const int64_t cost = rounds * ((p.kslice + kw - 1) / kw + (kw > 1 ? 2 : 1));
@@ -560,11 +660,16 @@ static W4Plan w4_plan(int64_t M, int64_t N, int64_t K, int group, bool f32) {
   }
   const int64_t blocks = (items * p.kw + p.warps - 1) / p.warps;
   p.grid_x = (int)(blocks < slots ? (blocks > 0 ? blocks : 1) : slots);
-  p.bytes = p.slices > 1 ? (int64_t)p.slices * M * N * 4 : 0;
+  p.image = p.prepare ? p.grid_y * w4_image_bytes(KT, p.rows * per, gs, p.nt) : 0;
+  p.bytes = p.image + (p.slices > 1 ? (int64_t)p.slices * M * N * 4 : 0);
   return p;
 }
 
 template <int NT, int GS> static void w4_launch(const W4Args& a, const W4Plan& p, cudaStream_t st) {
+  if (p.prepare) {
+    const int64_t eights = (int64_t)p.rows * a.w.ktiles() * 16;
+    launch_pdl(w4_x_kernel<GS>, dim3((unsigned)((eights + 255) / 256), p.grid_y), dim3(256), 0, st, a, NT);
+  }
   auto kern = w4_kernel<NT, GS>;
   allow_max_dynamic_smem(kern);
   launch_pdl(kern, dim3(p.grid_x, p.grid_y, p.slices), dim3(32 * p.warps), (size_t)p.smem, st, a);
@@ -668,8 +773,7 @@ extern "C" int b2k_w4_matmul(const void* x, int64_t ldx, int xtype, const float*
   a.xtype = xtype; a.ytype = ytype; a.stype = stype;
   const W4Plan p = w4_plan(M, N, K, group, xtype == B2K_F32);
   B2K_REQUIRE(p.grid_y <= 65535 && p.slices <= 65535, "b2k_w4_matmul: shape too large");
-  B2K_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes &&
-                               (reinterpret_cast<uintptr_t>(workspace) & 3u) == 0),
+  B2K_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes && aligned16(workspace)),
               "b2k_w4_matmul: the workspace needs %lld bytes, got %lld", (long long)p.bytes,
               (long long)workspace_bytes);
   const int xsize = dtype_size(xtype);
@@ -677,7 +781,10 @@ extern "C" int b2k_w4_matmul(const void* x, int64_t ldx, int xtype, const float*
   a.x_aligned = reinterpret_cast<uintptr_t>(x) % (xsize == 1 ? 8 : 16) == 0 &&
                 ldx * xsize % (xsize == 1 ? 8 : 16) == 0;
   a.KW = p.kw; a.kslice = p.kslice; a.rows = p.rows;
-  a.part = p.bytes ? static_cast<float*>(workspace) : nullptr;
+  a.stages = p.stages;
+  a.xw = p.prepare ? static_cast<unsigned char*>(workspace) : nullptr;
+  a.part = p.slices > 1 ? reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + p.image)
+                        : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (p.nt == 1) w4_dispatch<1>(a, p, st);
   else if (p.nt == 2) w4_dispatch<2>(a, p, st);
