@@ -340,8 +340,9 @@ __global__ void __launch_bounds__(256) w4_x_kernel(const __grid_constant__ W4Arg
       go[(int64_t)(v8 / (16 / GS)) * 8 * nt + col] = f2(0.0f, 0.0f);
 }
 
-// GS = groups per 128 columns, 8 NT = columns (rows of x; two each for float32)
-template <int NT, int GS> __global__ void __launch_bounds__(512, 1) w4_kernel(
+// GS = groups per 128 columns, 8 NT = columns (rows of x; two each for
+// float32), BF: scales and zeros are bfloat16
+template <int NT, int GS, bool BF> __global__ void __launch_bounds__(512, 1) w4_kernel(
     const __grid_constant__ W4Args a) {
   constexpr int RT = w4_rt(NT), SBK = w4_sbk(NT), G = 128 / GS, STAGE = w4_stage(GS);
   const int S = a.stages;
@@ -360,6 +361,7 @@ template <int NT, int GS> __global__ void __launch_bounds__(512, 1) w4_kernel(
   unsigned char* ring = smem + warp * (S * STAGE);
   unsigned char* xsm = smem + nwarps * (S * STAGE);
   float2* gsm = reinterpret_cast<float2*>(xsm + w4_x_bytes(a.kslice, f32 ? 2 * a.rows : a.rows));
+  __shared__ uint4 nothing;  // what lanes past the last column read
 
   // ---- this warp's stream of weights ---------------------------------------
   const int KW = a.KW, kw = warp % KW, grp = warp / KW, groups = nwarps / KW;
@@ -371,6 +373,18 @@ template <int NT, int GS> __global__ void __launch_bounds__(512, 1) w4_kernel(
   int pk = k0, get_stage = 0, use_stage = 0;
   uint32_t use_phase = 0, issued = 0, used = 0;
   bool dead = false;  // a wait ran out
+  // the next bytes of the item's (first) tile, and how far its second one is
+  const unsigned char *wsrc = nullptr, *ssrc = nullptr, *zsrc = nullptr;
+  int64_t wnext = 0;
+  auto open = [&]() {
+    const int64_t at = pit * RT * KT + kb0 + k0;
+    wsrc = a.w.tiles + at * 1024;
+    ssrc = static_cast<const unsigned char*>(a.w.scales) + at * GS * 32;
+    if (zeros) zsrc = static_cast<const unsigned char*>(a.w.zeros) + at * GS * 32;
+    // past the last tile the first is read again
+    wnext = RT > 1 && pit * RT + 1 < tiles ? KT : 0;
+    pk = k0;
+  };
   auto issue = [&]() {
     const int n = min(SBK, k1 - pk);
     if (lane == 0) {
@@ -381,35 +395,36 @@ template <int NT, int GS> __global__ void __launch_bounds__(512, 1) w4_kernel(
       mbar_arrive_expect_tx(bar, RT * (wb + (zeros ? 2 : 1) * sb));
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        const int64_t at = min(pit * RT + t, tiles - 1) * KT + kb0 + pk;
-        bulk_g2s(dst + t * SBK * 1024, a.w.tiles + at * 1024, wb, bar);
-        bulk_g2s(dst + 2048 + t * SBK * GS * 32,
-                 static_cast<const unsigned char*>(a.w.scales) + at * GS * 32, sb, bar);
+        bulk_g2s(dst + t * SBK * 1024, wsrc + t * wnext * 1024, wb, bar);
+        bulk_g2s(dst + 2048 + t * SBK * GS * 32, ssrc + t * wnext * GS * 32, sb, bar);
         if (zeros)
-          bulk_g2s(dst + 2048 + (2 * GS + t * SBK * GS) * 32,
-                   static_cast<const unsigned char*>(a.w.zeros) + at * GS * 32, sb, bar);
+          bulk_g2s(dst + 2048 + (2 * GS + t * SBK * GS) * 32, zsrc + t * wnext * GS * 32, sb, bar);
       }
     }
     if (++get_stage == S) get_stage = 0;
     ++issued;
-    pk += n;
+    wsrc += SBK * 1024;
+    ssrc += SBK * GS * 32;
+    zsrc += SBK * GS * 32;
+    pk += SBK;
     if (pk >= k1) {
-      pk = k0;
       pit += step;
+      open();
     }
   };
   griddep_launch_dependents();
   if (lane < S) mbar_init(&full[warp][lane], 1);
+  if (tid == 0) nothing = zero4();
   fence_barrier_init();
   __syncwarp();
   // With x prepared by the kernel before, the weights need not wait for it.
   if (!a.xw) griddep_wait();
+  open();
   if (k0 < k1)
     for (int s = 0; s < S && pit < items; ++s) issue();
   if (a.xw) griddep_wait();
 
   // ---- x into shared memory -------------------------------------------------
-  for (int i = tid; i < kn * GS * 8 * NT; i += blockDim.x) gsm[i] = f2(0.0f, 0.0f);
   if (a.xw) {  // prepared by w4_x_kernel
     if (tid == 0) {
       mbar_init(&xbar, 1);
@@ -430,6 +445,7 @@ template <int NT, int GS> __global__ void __launch_bounds__(512, 1) w4_kernel(
       if (lane == 0) atomicAdd(&b2k_tu_timeouts, 1u);
     }
   } else {
+    for (int i = tid; i < kn * GS * 8 * NT; i += blockDim.x) gsm[i] = f2(0.0f, 0.0f);
     __syncthreads();
     const int per_row = kn * 16, total = rows * per_row;  // eights of columns
     for (int base = warp * 32; base < total; base += blockDim.x) {
@@ -498,6 +514,15 @@ template <int NT, int GS> __global__ void __launch_bounds__(512, 1) w4_kernel(
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[t][nt][e] = 0.0f;
   const uint32_t swap = odd ? 0x1032u : 0x3210u;
+  // this lane's fragments of x: where, and from one 32 columns to the next
+  const unsigned char* xat[NT];
+  int xstep[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const bool in = nt * 8 + r < C;
+    xat[nt] = in ? xsm + (nt * 8 + r) * 64 + c * 16 : reinterpret_cast<const unsigned char*>(&nothing);
+    xstep[nt] = in ? C * 64 : 0;
+  }
 
   for (int64_t it = first; it < items; it += step) {
     int stage = 0;
@@ -527,11 +552,9 @@ template <int NT, int GS> __global__ void __launch_bounds__(512, 1) w4_kernel(
         float acc[RT][NT][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const unsigned char* xp = xsm + (int64_t)(4 * (k + i) + j) * C * 64 + r * 64 + c * 16;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            uint4 b = zero4();
-            if (nt * 8 + r < C) b = *reinterpret_cast<const uint4*>(xp + nt * 512);
+            const uint4 b = *reinterpret_cast<const uint4*>(xat[nt] + (4 * (k + i) + j) * xstep[nt]);
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
               const uint32_t w0 = j == 0 ? wa[t].x : j == 1 ? wa[t].y : j == 2 ? wa[t].z : wa[t].w;
@@ -549,7 +572,7 @@ template <int NT, int GS> __global__ void __launch_bounds__(512, 1) w4_kernel(
           }
           if ((j + 1) * 32 % G == 0) {
             const int gi = j * 32 / G;
-            const float4* gp = reinterpret_cast<const float4*>(gsm + ((k + i) * GS + gi) * 8 * NT + 2 * c);
+            const float4* gp = reinterpret_cast<const float4*>(gsm + ((k + i) * GS + gi) * (8 * NT) + 2 * c);
             float4 g4[NT];  // (sum, scale) of columns 2c, 2c + 1
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) g4[nt] = gp[nt * 4];
@@ -560,8 +583,8 @@ template <int NT, int GS> __global__ void __launch_bounds__(512, 1) w4_kernel(
                   st + 2048 + ((t * SBK + i) * GS + gi) * 32) + r;
               auto two = [&](uint32_t bits) {
                 bits = __byte_perm(bits, 0, swap);
-                if (a.stype == B2K_F16) return __half22float2(*reinterpret_cast<const __half2*>(&bits));
-                return f2(__uint_as_float(bits << 16), __uint_as_float(bits & 0xffff0000u));
+                if constexpr (!BF) return __half22float2(*reinterpret_cast<const __half2*>(&bits));
+                else return f2(__uint_as_float(bits << 16), __uint_as_float(bits & 0xffff0000u));
               };
               const float2 z = zeros ? two(sp[2 * GS * 8]) : f2s(8.0f);
               // 2^10: 2^24 of the integers' unit, 2^-14 of x's
@@ -613,8 +636,8 @@ template <typename T> __global__ void __launch_bounds__(256) w4_sum_kernel(const
 // where x does not fit beside two.  x is prepared once by a kernel of its own
 // where every block's own preparation would take it more than kW4Own eights of
 // columns per thread.  KW is the number of warps per tile that leaves the
-// longest warp the least to do, counting a tile's join as two blocks of 128
-// columns.
+// longest warp the least to do, counting the join of an item as half of a block
+// of 128 columns of two tiles.
 constexpr int kW4Own = 4;
 struct W4Plan {
   int nt, rows, warps, stages, kslice, slices, kw, grid_x, grid_y;
@@ -652,7 +675,7 @@ static W4Plan w4_plan(int64_t M, int64_t N, int64_t K, int group, bool f32) {
   p.kw = 1;
   for (int kw = 1; kw <= p.warps; kw <<= 1) {
     const int64_t rounds = (items * kw + slots * p.warps - 1) / (slots * p.warps);
-    const int64_t cost = rounds * ((p.kslice + kw - 1) / kw + (kw > 1 ? 2 : 1));
+    const int64_t cost = rounds * (2 * ((p.kslice + kw - 1) / kw) + 2 / w4_rt(p.nt));
     if (best < 0 || cost < best) {
       best = cost;
       p.kw = kw;
@@ -665,22 +688,28 @@ static W4Plan w4_plan(int64_t M, int64_t N, int64_t K, int group, bool f32) {
   return p;
 }
 
-template <int NT, int GS> static void w4_launch(const W4Args& a, const W4Plan& p, cudaStream_t st) {
+template <int NT, int GS, bool BF> static void w4_launch(const W4Args& a, const W4Plan& p, cudaStream_t st) {
   if (p.prepare) {
     const int64_t eights = (int64_t)p.rows * a.w.ktiles() * 16;
     launch_pdl(w4_x_kernel<GS>, dim3((unsigned)((eights + 255) / 256), p.grid_y), dim3(256), 0, st, a, NT);
   }
-  auto kern = w4_kernel<NT, GS>;
+  auto kern = w4_kernel<NT, GS, BF>;
   allow_max_dynamic_smem(kern);
   launch_pdl(kern, dim3(p.grid_x, p.grid_y, p.slices), dim3(32 * p.warps), (size_t)p.smem, st, a);
 }
 
-template <int NT> static void w4_dispatch(const W4Args& a, const W4Plan& p, cudaStream_t st) {
+template <int NT, bool BF> static void w4_dispatch(const W4Args& a, const W4Plan& p, cudaStream_t st) {
   switch (a.w.g) {
-    case 32: w4_launch<NT, 4>(a, p, st); break;
-    case 64: w4_launch<NT, 2>(a, p, st); break;
-    default: w4_launch<NT, 1>(a, p, st); break;
+    case 32: w4_launch<NT, 4, BF>(a, p, st); break;
+    case 64: w4_launch<NT, 2, BF>(a, p, st); break;
+    default: w4_launch<NT, 1, BF>(a, p, st); break;
   }
+}
+
+template <bool BF> static void w4_columns(const W4Args& a, const W4Plan& p, cudaStream_t st) {
+  if (p.nt == 1) w4_dispatch<1, BF>(a, p, st);
+  else if (p.nt == 2) w4_dispatch<2, BF>(a, p, st);
+  else w4_dispatch<4, BF>(a, p, st);
 }
 
 static int w4_check(const char* what, int64_t N, int64_t K, int group, int stype) {
@@ -786,9 +815,8 @@ extern "C" int b2k_w4_matmul(const void* x, int64_t ldx, int xtype, const float*
   a.part = p.slices > 1 ? reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + p.image)
                         : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (p.nt == 1) w4_dispatch<1>(a, p, st);
-  else if (p.nt == 2) w4_dispatch<2>(a, p, st);
-  else w4_dispatch<4>(a, p, st);
+  if (stype == B2K_F16) w4_columns<false>(a, p, st);
+  else w4_columns<true>(a, p, st);
   if (a.part) {
     const unsigned grid = w4_blocks(M * N);
     B2K_DISPATCH_FLOAT(ytype, {
