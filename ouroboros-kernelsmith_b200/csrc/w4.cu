@@ -10,6 +10,7 @@
 // bits 4i .. 4i+3).  Scales and zeros: [ceil(N/16), ceil(K/128), 128/g, 16].
 // Rows and columns past N and K hold zeros with scale zero.
 #include <cuda_fp8.h>
+#include <limits.h>
 
 #include "rowio.cuh"
 #include "rowpipe.cuh"
@@ -136,9 +137,10 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const T* w, int64_t ld
 // (22 bits).  8-bit x is exact as it is and xs is its scale.
 //
 // Blocks are persistent, one per SM, and hold all of x (their slice of K) in
-// shared memory, prepared once.  KW warps share a row tile, each with a run of
-// its blocks of 128 columns; every warp has its own ring of bulk copies, which
-// runs ahead across tiles.
+// shared memory, prepared once.  A block takes an equal share of the row tiles
+// and its warps equal runs of their blocks of 128 columns, whatever tile these
+// lie in; a tile that spans warps is added up at the end.  Every warp has its
+// own ring of bulk copies, which runs ahead across tiles.
 constexpr int kW4Stages = 4, kW4Smem = 226 << 10;  // stages at most; of an SM's memory
 
 struct W4Args {
@@ -151,9 +153,9 @@ struct W4Args {
   void* y;
   int64_t ldy, M;
   int xtype, ytype, stype, x_aligned;
-  int KW;          // warps that share a row tile
   int kslice;      // blocks of 128 columns per grid.z
   int rows;        // rows of x per grid.y
+  int64_t each, more;  // items of a block; one more in the first `more`
   int stages;      // of a warp's ring
   unsigned char* xw;  // x prepared by w4_x_kernel (null: each block prepares its own)
   float* part;     // [grid.z][M][N] partial sums when K is split over blocks
@@ -207,7 +209,7 @@ __device__ __forceinline__ uint32_t h2_bits(__half a, __half b) {
 
 __device__ __forceinline__ void w4_mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                        uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -217,7 +219,7 @@ __device__ __forceinline__ void w4_mma(float* c, uint32_t a0, uint32_t a1, uint3
 // the same on zero sums
 __device__ __forceinline__ void w4_mma_first(float* c, uint32_t a0, uint32_t a1, uint32_t a2,
                                              uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%10,%10,%10,%10};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
@@ -227,8 +229,10 @@ __device__ __forceinline__ void w4_mma_first(float* c, uint32_t a0, uint32_t a1,
 // row tiles of 16 per warp: x's fragments are read once for all of them, which
 // with 16 columns and more would otherwise take more of shared memory's
 // bandwidth than the weights; and blocks of 128 columns in a stage of the ring
-__host__ __device__ constexpr int w4_rt(int NT) { return NT == 1 ? 1 : 2; }
+__host__ __device__ constexpr int w4_rt(int NT) { return NT <= 2 ? 1 : 2; }
 __host__ __device__ constexpr int w4_sbk(int NT) { return 2 / w4_rt(NT); }
+// warps of a block: 32 columns need the registers of 8
+__host__ __device__ constexpr int w4_warps(int NT) { return NT == 4 ? 8 : 16; }
 // stage: 2 KB of weights, then the scales and the zeros of their groups
 __host__ __device__ constexpr int w4_stage(int gs) { return 2048 + 128 * gs; }
 // bytes of x, and of its groups' sums and scales, for kslice blocks of columns;
@@ -342,15 +346,13 @@ __global__ void __launch_bounds__(256) w4_x_kernel(const __grid_constant__ W4Arg
 
 // GS = groups per 128 columns, 8 NT = columns (rows of x; two each for
 // float32), BF: scales and zeros are bfloat16
-template <int NT, int GS, bool BF> __global__ void __launch_bounds__(512, 1) w4_kernel(
+template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * w4_warps(NT), 1) w4_kernel(
     const __grid_constant__ W4Args a) {
-  constexpr int RT = w4_rt(NT), SBK = w4_sbk(NT), G = 128 / GS, STAGE = w4_stage(GS);
+  constexpr int RT = w4_rt(NT), SBK = w4_sbk(NT), G = 128 / GS, STAGE = w4_stage(GS), W = w4_warps(NT);
   const int S = a.stages;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint64_t full[16][kW4Stages], xbar;
-  __shared__ int red_at[16];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
-  const int nwarps = blockDim.x >> 5;
   const int64_t KT = a.w.ktiles(), tiles = a.w.ntiles();
   const int64_t kb0 = (int64_t)blockIdx.z * a.kslice;
   const int kn = (int)min((int64_t)a.kslice, KT - kb0);  // blocks of this slice
@@ -359,35 +361,62 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(512, 1) w4_
   const bool f32 = a.xtype == B2K_F32, zeros = a.w.zeros != nullptr;
   const int C = f32 ? 2 * rows : rows;
   unsigned char* ring = smem + warp * (S * STAGE);
-  unsigned char* xsm = smem + nwarps * (S * STAGE);
+  unsigned char* xsm = smem + W * (S * STAGE);
   float2* gsm = reinterpret_cast<float2*>(xsm + w4_x_bytes(a.kslice, f32 ? 2 * a.rows : a.rows));
   __shared__ uint4 nothing;  // what lanes past the last column read
 
-  // ---- this warp's stream of weights ---------------------------------------
-  const int KW = a.KW, kw = warp % KW, grp = warp / KW, groups = nwarps / KW;
-  const int chunk = (kn + KW - 1) / KW;
-  const int k0 = min(kn, kw * chunk), k1 = min(kn, k0 + chunk);  // its blocks
-  const int64_t items = (tiles + RT - 1) / RT, step = (int64_t)gridDim.x * groups;
-  const int64_t first = (int64_t)blockIdx.x * groups + grp;
-  int64_t pit = first;  // next to load
-  int pk = k0, get_stage = 0, use_stage = 0;
+  // ---- this warp's run of blocks --------------------------------------------
+  // The block's items (RT row tiles each) laid end to end, kn blocks of columns
+  // apiece, and divided into equal runs.  A run's whole items are taken first,
+  // then the end of the run that begins another item (its tail), last its head,
+  // the end of an item that an earlier warp begins.
+  const int64_t b = blockIdx.x;
+  const int64_t i0 = b * a.each + min(b, a.more);        // its items: the first
+  const int n_items = (int)(a.each + (b < a.more));      // and their number
+  const int64_t units = (int64_t)n_items * kn;
+  auto run_at = [&](int w) { return (int)(w * units / W); };
+  const int u0 = run_at(warp), u1 = run_at(warp + 1);
+  // whole items before the run's first item boundary, and where that lies
+  const int before = kn > 0 ? (int)((uint32_t)(u0 + kn - 1) / (uint32_t)kn) : 0;
+  const int body = min(u1, before * kn);
+
+  // a walk over the run: blocks [k, end) of item i0 + item
+  struct Walk {
+    int item, k, end, at;  // at: the units up to here, past u1 after the head
+  };
+  // the next item of the walk; false after the last
+  auto next_item = [&](Walk& w) {
+    if (w.at < u1 && w.at >= body) {
+      w.k = 0;
+      w.end = min(kn, u1 - w.at);
+      w.at += w.end;
+      return true;
+    }
+    if (w.at == u1 && u0 < body) {  // from the body to the head
+      w.item = before - 1;
+      w.k = u0 - w.item * kn;
+      w.end = w.k + body - u0;
+      w.at = INT_MAX;
+      return true;
+    }
+    return false;
+  };
+  const Walk begin = {before, 0, 0, body};
+  Walk get = begin;
+  int get_stage = 0, use_stage = 0;
   uint32_t use_phase = 0, issued = 0, used = 0;
   bool dead = false;  // a wait ran out
-  // the next bytes of the item's (first) tile, and how far its second one is
-  const unsigned char *wsrc = nullptr, *ssrc = nullptr, *zsrc = nullptr;
-  int64_t wnext = 0;
+  int64_t get_at = 0;  // block of the item's (first) tile in the layout
+  int get_left = 0;    // blocks of it to come
+  bool getting = false;
   auto open = [&]() {
-    const int64_t at = pit * RT * KT + kb0 + k0;
-    wsrc = a.w.tiles + at * 1024;
-    ssrc = static_cast<const unsigned char*>(a.w.scales) + at * GS * 32;
-    if (zeros) zsrc = static_cast<const unsigned char*>(a.w.zeros) + at * GS * 32;
-    // past the last tile the first is read again
-    wnext = RT > 1 && pit * RT + 1 < tiles ? KT : 0;
-    pk = k0;
+    getting = u0 < u1 && next_item(get);
+    get_at = (i0 + get.item) * RT * KT + kb0 + get.k;
+    get_left = get.end - get.k;
   };
   auto issue = [&]() {
-    const int n = min(SBK, k1 - pk);
     if (lane == 0) {
+      const int n = min(SBK, get_left);
       uint64_t* bar = &full[warp][get_stage];
       unsigned char* dst = ring + get_stage * STAGE;
       const uint32_t wb = n * 1024, sb = n * GS * 32;
@@ -395,20 +424,22 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(512, 1) w4_
       mbar_arrive_expect_tx(bar, RT * (wb + (zeros ? 2 : 1) * sb));
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        bulk_g2s(dst + t * SBK * 1024, wsrc + t * wnext * 1024, wb, bar);
-        bulk_g2s(dst + 2048 + t * SBK * GS * 32, ssrc + t * wnext * GS * 32, sb, bar);
+        // past the last tile the first is read again
+        const int64_t at = t == 0 || (i0 + get.item) * RT + t >= tiles ? get_at : get_at + t * KT;
+        bulk_g2s(dst + t * SBK * 1024, a.w.tiles + at * 1024, wb, bar);
+        bulk_g2s(dst + 2048 + t * SBK * GS * 32,
+                 static_cast<const unsigned char*>(a.w.scales) + at * GS * 32, sb, bar);
         if (zeros)
-          bulk_g2s(dst + 2048 + (2 * GS + t * SBK * GS) * 32, zsrc + t * wnext * GS * 32, sb, bar);
+          bulk_g2s(dst + 2048 + (2 * GS + t * SBK * GS) * 32,
+                   static_cast<const unsigned char*>(a.w.zeros) + at * GS * 32, sb, bar);
       }
     }
     if (++get_stage == S) get_stage = 0;
     ++issued;
-    wsrc += SBK * 1024;
-    ssrc += SBK * GS * 32;
-    zsrc += SBK * GS * 32;
-    pk += SBK;
-    if (pk >= k1) {
-      pit += step;
+    get_at += SBK;
+    get_left -= SBK;
+    if (get_left <= 0) {
+      ++get.item;
       open();
     }
   };
@@ -420,8 +451,7 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(512, 1) w4_
   // With x prepared by the kernel before, the weights need not wait for it.
   if (!a.xw) griddep_wait();
   open();
-  if (k0 < k1)
-    for (int s = 0; s < S && pit < items; ++s) issue();
+  for (int s = 0; s < S && getting; ++s) issue();
   if (a.xw) griddep_wait();
 
   // ---- x into shared memory -------------------------------------------------
@@ -455,56 +485,21 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(512, 1) w4_
     __syncthreads();
   }
 
-  // ---- the group's warps add up a tile; its rows are columns of y ------------
-  // Their parts lie in the stages that they have just read.
+  // ---- results ----------------------------------------------------------------
   const int odd = r & 1, row_a = 2 * r + odd, row_b = 2 * r + 1 - odd;  // rows r, r + 8 of the products
-  auto sync_group = [&]() {
-    if (KW > 1) named_bar_sync(1 + grp, 32 * KW);
-    else __syncwarp();
-  };
-  auto join = [&](int64_t it, int stage, float (&y)[RT][NT][4]) {
-    if (lane == 0) red_at[warp] = warp * (S * STAGE) + stage * STAGE;
-    float* mine = reinterpret_cast<float*>(ring + stage * STAGE);  // [column][16 rows]
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      __syncwarp();  // this warp has read the stage
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          mine[(nt * 8 + 2 * c + (e & 1)) * 16 + (e >> 1 ? row_b : row_a)] = y[t][nt][e];
-          y[t][nt][e] = 0.0f;
-        }
-      sync_group();
-      for (int i = kw * 32 + lane; i < rows * 16; i += 32 * KW) {
-        const int m = i >> 4, n16 = i & 15;
-        const int64_t n = (it * RT + t) * 16 + n16;
-        if (n >= a.w.N) continue;
-        float v = 0.0f;
-        if (f32) {
-          float lo = 0.0f;
-          for (int w = 0; w < KW; ++w) {
-            const float* from = reinterpret_cast<const float*>(smem + red_at[grp * KW + w]);
-            v += from[2 * m * 16 + n16];
-            lo += from[(2 * m + 1) * 16 + n16];
-          }
-          v = fmaf(lo, 0.00048828125f, v);
-        } else {
-          for (int w = 0; w < KW; ++w)
-            v += reinterpret_cast<const float*>(smem + red_at[grp * KW + w])[i];
-        }
-        if (a.part) {
-          a.part[((int64_t)blockIdx.z * a.M + m0 + m) * a.w.N + n] = v;
-          continue;
-        }
-        const int64_t at = (m0 + m) * a.ldy + n;
-        if (a.ytype == B2K_F32) static_cast<float*>(a.y)[at] = v;
-        else if (a.ytype == B2K_F16) static_cast<__half*>(a.y)[at] = from_f<__half>(v);
-        else static_cast<__nv_bfloat16*>(a.y)[at] = from_f<__nv_bfloat16>(v);
-      }
-      sync_group();
+  // column n of row m of y (of the partial sums when K is split)
+  auto store = [&](int m, int64_t n, float v) {
+    if (n >= a.w.N) return;
+    if (a.part) {
+      a.part[((int64_t)blockIdx.z * a.M + m0 + m) * a.w.N + n] = v;
+      return;
     }
+    const int64_t at = (m0 + m) * a.ldy + n;
+    if (a.ytype == B2K_F32) static_cast<float*>(a.y)[at] = v;
+    else if (a.ytype == B2K_F16) static_cast<__half*>(a.y)[at] = from_f<__half>(v);
+    else static_cast<__nv_bfloat16*>(a.y)[at] = from_f<__nv_bfloat16>(v);
   };
+  constexpr float kLow = 0.00048828125f;  // 2^-11, the weight of float32's second column
 
   float y[RT][NT][4];
 #pragma unroll
@@ -524,9 +519,12 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(512, 1) w4_
     xstep[nt] = in ? C * 64 : 0;
   }
 
-  for (int64_t it = first; it < items; it += step) {
+  float tail[RT][NT][4];  // of the item that the run begins and does not end
+  int tail_item = -1;
+  Walk use = begin;
+  while (u0 < u1 && next_item(use)) {
     int stage = 0;
-    for (int k = k0; k < k1; k += SBK) {
+    for (int k = use.k; k < use.end; k += SBK) {
       stage = use_stage;
       if (!dead && !mbar_wait(&full[warp][stage], use_phase)) {
         // stay in step with the group's barriers; the results are lost
@@ -541,7 +539,7 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(512, 1) w4_
       const unsigned char* st = ring + stage * STAGE;
 #pragma unroll
       for (int i = 0; i < SBK; ++i) {
-        if (SBK > 1 && k + i >= k1) break;
+        if (SBK > 1 && k + i >= use.end) break;
         uint4 wa[RT], wb[RT];
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
@@ -602,19 +600,89 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(512, 1) w4_
           }
         }
       }
-      if (k + SBK < k1) {  // the last stage of a tile is needed for the join
-        __syncwarp();
-        if (!dead && pit < items) issue();
-      }
+      __syncwarp();
+      if (getting && !dead) issue();
     }
-    join(it, stage, y);
-    if (k0 < k1 && !dead && pit < items) issue();
+    if (use.at == INT_MAX) break;  // the head stays in y
+    const bool ends = use.end == kn;
+    const int64_t item = i0 + use.item;
+    ++use.item;
+    if (!ends) {
+      tail_item = use.item - 1;
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) tail[t][nt][e] = y[t][nt][e];
+    } else {
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int64_t n = (item * RT + t) * 16 + (h ? row_b : row_a);
+            const float v0 = y[t][nt][2 * h], v1 = y[t][nt][2 * h + 1];
+            const int col = nt * 8 + 2 * c;
+            if (f32) {
+              if (col < C) store(col >> 1, n, fmaf(v1, kLow, v0));
+            } else {
+              if (col < C) store(col, n, v0);
+              if (col + 1 < C) store(col + 1, n, v1);
+            }
+          }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[t][nt][e] = 0.0f;
   }
-  if (dead)  // nothing may land after the block has gone
-    for (; used <= issued && used > 0; ++used) {
-      const uint32_t t = used - 1;  // the tile that was given up, and those after it
-      if (t < issued) mbar_wait(&full[warp][t % S], (t / S) & 1);
+  if (dead)  // nothing may land where the parts go
+    for (used -= used > 0; used < issued; ++used)
+      mbar_wait(&full[warp][used % S], (used / S) & 1);
+
+  // ---- items that span warps: their parts, in the warps' drained rings ----------
+  if (kn == 0) {  // no columns at all
+    for (int64_t i = tid; i < (int64_t)n_items * RT * 16 * rows; i += blockDim.x)
+      store((int)(i % rows), i0 * RT * 16 + i / rows, 0.0f);
+    return;
+  }
+  constexpr int PER = RT * 16 * 8 * NT;
+  const bool has_tail = tail_item >= 0;
+  __syncwarp();
+  float* mine = reinterpret_cast<float*>(ring);  // [head, tail][column][RT * 16 rows]
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = (nt * 8 + 2 * c + (e & 1)) * RT * 16 + t * 16 + (e >> 1 ? row_b : row_a);
+        mine[at] = y[t][nt][e];  // zeros where there is no head
+        if (has_tail) mine[PER + at] = tail[t][nt][e];
+      }
+  __syncthreads();
+  // this warp's tail, and the heads of the next warps whose runs lie in that item
+  if (!has_tail) return;
+  const int past = (tail_item + 1) * kn;
+  int last = warp;
+#pragma unroll
+  for (int w = 1; w < W; ++w) last += w > warp && run_at(w) < past;
+  for (int i = lane; i < rows * RT * 16; i += 32) {
+    const int m = i / (RT * 16), n16 = i - m * RT * 16;
+    const int c0 = (f32 ? 2 * m : m) * RT * 16 + n16, c1 = f32 ? c0 + RT * 16 : c0;
+    float v = mine[PER + c0], low = mine[PER + c1];
+    const float* from = reinterpret_cast<const float*>(smem);
+#pragma unroll 4
+    for (int w = warp + 1; w <= last; ++w) {
+      v += from[w * (S * STAGE / 4) + c0];
+      low += from[w * (S * STAGE / 4) + c1];
     }
+    store(m, (i0 + tail_item) * RT * 16 + n16, f32 ? fmaf(low, kLow, v) : v);
+  }
 }
 
 // y = the sum of K's slices, in order
@@ -631,18 +699,16 @@ template <typename T> __global__ void __launch_bounds__(256) w4_sum_kernel(const
   }
 }
 
-// How a product is split.  One block of 16 warps per SM, their rings as deep as
-// shared memory allows beside x (2 to kW4Stages stages); K is split over blocks
-// where x does not fit beside two.  x is prepared once by a kernel of its own
-// where every block's own preparation would take it more than kW4Own eights of
-// columns per thread.  KW is the number of warps per tile that leaves the
-// longest warp the least to do, counting the join of an item as half of a block
-// of 128 columns of two tiles.
+// How a product is split.  One block per SM, its warps' rings as deep as shared
+// memory allows beside x (kW4Stages stages at most, and two parts of an item at
+// least); K is split over blocks where x does not fit beside that.  x is
+// prepared once by a kernel of its own where every block's own preparation
+// would take it more than kW4Own eights of columns per thread.
 constexpr int kW4Own = 4;
 struct W4Plan {
-  int nt, rows, warps, stages, kslice, slices, kw, grid_x, grid_y;
+  int nt, rows, warps, stages, kslice, slices, grid_x, grid_y;
   bool prepare;
-  int64_t smem, image, bytes;
+  int64_t smem, image, bytes, each, more;
 };
 
 static W4Plan w4_plan(int64_t M, int64_t N, int64_t K, int group, bool f32) {
@@ -652,14 +718,15 @@ static W4Plan w4_plan(int64_t M, int64_t N, int64_t K, int group, bool f32) {
   p.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
   p.rows = (int)(M < 8 * p.nt / per ? M : 8 * p.nt / per);
   p.grid_y = (int)((M + p.rows - 1) / p.rows);
-  p.warps = 16;
+  p.warps = w4_warps(p.nt);
+  const int least = p.nt == 4 ? 4 : 2;  // 2 PER floats fit these stages
   auto need = [&](int64_t kslice, int stages) {
     return w4_x_bytes(kslice, p.rows * per) + w4_g_bytes(kslice, gs, p.nt) +
            (int64_t)p.warps * stages * w4_stage(gs);
   };
   p.slices = 1;
   p.kslice = (int)(KT > 0 ? KT : 1);
-  while (need(p.kslice, 2) > kW4Smem) {
+  while (need(p.kslice, least) > kW4Smem) {
     ++p.slices;
     p.kslice = (int)((KT + p.slices - 1) / p.slices);
   }
@@ -671,18 +738,9 @@ static W4Plan w4_plan(int64_t M, int64_t N, int64_t K, int group, bool f32) {
   const int64_t items = (tiles + w4_rt(p.nt) - 1) / w4_rt(p.nt);
   int64_t slots = (int64_t)sm_count() / (p.slices * p.grid_y);
   if (slots < 1) slots = 1;
-  int64_t best = -1;
-  p.kw = 1;
-  for (int kw = 1; kw <= p.warps; kw <<= 1) {
-    const int64_t rounds = (items * kw + slots * p.warps - 1) / (slots * p.warps);
-    const int64_t cost = rounds * (2 * ((p.kslice + kw - 1) / kw) + 2 / w4_rt(p.nt));
-    if (best < 0 || cost < best) {
-      best = cost;
-      p.kw = kw;
-    }
-  }
-  const int64_t blocks = (items * p.kw + p.warps - 1) / p.warps;
-  p.grid_x = (int)(blocks < slots ? (blocks > 0 ? blocks : 1) : slots);
+  p.grid_x = (int)(items < slots ? items : slots);
+  p.each = items / p.grid_x;
+  p.more = items % p.grid_x;
   p.image = p.prepare ? p.grid_y * w4_image_bytes(KT, p.rows * per, gs, p.nt) : 0;
   p.bytes = p.image + (p.slices > 1 ? (int64_t)p.slices * M * N * 4 : 0);
   return p;
@@ -809,8 +867,8 @@ extern "C" int b2k_w4_matmul(const void* x, int64_t ldx, int xtype, const float*
   // eight columns are read as 16-byte vectors (8 bytes for 8-bit x)
   a.x_aligned = reinterpret_cast<uintptr_t>(x) % (xsize == 1 ? 8 : 16) == 0 &&
                 ldx * xsize % (xsize == 1 ? 8 : 16) == 0;
-  a.KW = p.kw; a.kslice = p.kslice; a.rows = p.rows;
-  a.stages = p.stages;
+  a.kslice = p.kslice; a.rows = p.rows;
+  a.stages = p.stages; a.each = p.each; a.more = p.more;
   a.xw = p.prepare ? static_cast<unsigned char*>(workspace) : nullptr;
   a.part = p.slices > 1 ? reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + p.image)
                         : nullptr;
