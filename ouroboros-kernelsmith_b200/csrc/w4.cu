@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const T* w, int64_t ld
 // -------------------------------------------------------------- the product
 //
 // Bound by reading the weights, N K / 2 bytes, while M is small.  A warp takes
-// 16 weight rows (or twice that) as the 16 rows of mma.m16n8k16, the rows of
+// 16 weight rows as the 16 rows of mma.m16n8k16, the rows of
 // x as its columns: the words of a tile are unpacked straight into A operands
 // (`word & 0x000f000f` is a pair of float16 subnormals n 2^-24, exact; `&
 // 0x00f000f0` 16 times that, against x / 16) and meet x from shared memory.
@@ -226,13 +226,8 @@ __device__ __forceinline__ void w4_mma_first(float* c, uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
-// row tiles of 16 per warp: x's fragments are read once for all of them, which
-// with 16 columns and more would otherwise take more of shared memory's
-// bandwidth than the weights; and blocks of 128 columns in a stage of the ring
-__host__ __device__ constexpr int w4_rt(int NT) { return NT <= 2 ? 1 : 2; }
-__host__ __device__ constexpr int w4_sbk(int NT) { return 2 / w4_rt(NT); }
-// warps of a block: 32 columns need the registers of 8
-__host__ __device__ constexpr int w4_warps(int NT) { return NT == 4 ? 8 : 16; }
+constexpr int kW4Warps = 16;  // of a block
+constexpr int kW4Blocks = 2;  // of 128 columns in a stage of a warp's ring
 // stage: 2 KB of weights, then the scales and the zeros of their groups
 __host__ __device__ constexpr int w4_stage(int gs) { return 2048 + 128 * gs; }
 // bytes of x, and of its groups' sums and scales, for kslice blocks of columns;
@@ -346,9 +341,10 @@ __global__ void __launch_bounds__(256) w4_x_kernel(const __grid_constant__ W4Arg
 
 // GS = groups per 128 columns, 8 NT = columns (rows of x; two each for
 // float32), BF: scales and zeros are bfloat16
-template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * w4_warps(NT), 1) w4_kernel(
+template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * kW4Warps, 1) w4_kernel(
     const __grid_constant__ W4Args a) {
-  constexpr int RT = w4_rt(NT), SBK = w4_sbk(NT), G = 128 / GS, STAGE = w4_stage(GS), W = w4_warps(NT);
+  constexpr int G = 128 / GS, STAGE = w4_stage(GS);
+  constexpr int SBK = kW4Blocks, W = kW4Warps;
   const int S = a.stages;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint64_t full[16][kW4Stages], xbar;
@@ -363,10 +359,12 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * w4_war
   unsigned char* ring = smem + warp * (S * STAGE);
   unsigned char* xsm = smem + W * (S * STAGE);
   float2* gsm = reinterpret_cast<float2*>(xsm + w4_x_bytes(a.kslice, f32 ? 2 * a.rows : a.rows));
-  __shared__ uint4 nothing;  // what lanes past the last column read
+  // 16 zero bytes, what lanes past the last column read
+  const uint32_t nothing = (uint32_t)(reinterpret_cast<unsigned char*>(gsm) - smem) +
+                           (uint32_t)w4_g_bytes(a.kslice, GS, NT);
 
   // ---- this warp's run of blocks --------------------------------------------
-  // The block's items (RT row tiles each) laid end to end, kn blocks of columns
+  // The block's items, its row tiles, laid end to end, kn blocks of columns
   // apiece, and divided into equal runs.  A run's whole items are taken first,
   // then the end of the run that begins another item (its tail), last its head,
   // the end of an item that an earlier warp begins.
@@ -411,7 +409,7 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * w4_war
   bool getting = false;
   auto open = [&]() {
     getting = u0 < u1 && next_item(get);
-    get_at = (i0 + get.item) * RT * KT + kb0 + get.k;
+    get_at = (i0 + get.item) * KT + kb0 + get.k;
     get_left = get.end - get.k;
   };
   auto issue = [&]() {
@@ -421,18 +419,13 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * w4_war
       unsigned char* dst = ring + get_stage * STAGE;
       const uint32_t wb = n * 1024, sb = n * GS * 32;
       fence_proxy_async();
-      mbar_arrive_expect_tx(bar, RT * (wb + (zeros ? 2 : 1) * sb));
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        // past the last tile the first is read again
-        const int64_t at = t == 0 || (i0 + get.item) * RT + t >= tiles ? get_at : get_at + t * KT;
-        bulk_g2s(dst + t * SBK * 1024, a.w.tiles + at * 1024, wb, bar);
-        bulk_g2s(dst + 2048 + t * SBK * GS * 32,
-                 static_cast<const unsigned char*>(a.w.scales) + at * GS * 32, sb, bar);
-        if (zeros)
-          bulk_g2s(dst + 2048 + (2 * GS + t * SBK * GS) * 32,
-                   static_cast<const unsigned char*>(a.w.zeros) + at * GS * 32, sb, bar);
-      }
+      mbar_arrive_expect_tx(bar, wb + (zeros ? 2 : 1) * sb);
+      bulk_g2s(dst, a.w.tiles + get_at * 1024, wb, bar);
+      bulk_g2s(dst + 2048, static_cast<const unsigned char*>(a.w.scales) + get_at * GS * 32,
+               sb, bar);
+      if (zeros)
+        bulk_g2s(dst + 2048 + SBK * GS * 32,
+                 static_cast<const unsigned char*>(a.w.zeros) + get_at * GS * 32, sb, bar);
     }
     if (++get_stage == S) get_stage = 0;
     ++issued;
@@ -445,7 +438,7 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * w4_war
   };
   griddep_launch_dependents();
   if (lane < S) mbar_init(&full[warp][lane], 1);
-  if (tid == 0) nothing = zero4();
+  if (tid == 0) *reinterpret_cast<uint4*>(smem + nothing) = zero4();
   fence_barrier_init();
   __syncwarp();
   // With x prepared by the kernel before, the weights need not wait for it.
@@ -501,33 +494,28 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * w4_war
   };
   constexpr float kLow = 0.00048828125f;  // 2^-11, the weight of float32's second column
 
-  float y[RT][NT][4];
-#pragma unroll
-  for (int t = 0; t < RT; ++t)
+  float y[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[t][nt][e] = 0.0f;
+      for (int e = 0; e < 4; ++e) y[nt][e] = 0.0f;
   const uint32_t swap = odd ? 0x1032u : 0x3210u;
   // this lane's fragments of x: where, and from one 32 columns to the next
-  const unsigned char* xat[NT];
-  int xstep[NT];
+  uint32_t xat[NT], xstep[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const bool in = nt * 8 + r < C;
-    xat[nt] = in ? xsm + (nt * 8 + r) * 64 + c * 16 : reinterpret_cast<const unsigned char*>(&nothing);
+    xat[nt] = in ? (uint32_t)(xsm - smem) + (nt * 8 + r) * 64 + c * 16 : nothing;
     xstep[nt] = in ? C * 64 : 0;
   }
-
-  float tail[RT][NT][4];  // of the item that the run begins and does not end
+  float tail[NT][4];  // of the item that the run begins and does not end
   int tail_item = -1;
   Walk use = begin;
   while (u0 < u1 && next_item(use)) {
-    int stage = 0;
     for (int k = use.k; k < use.end; k += SBK) {
-      stage = use_stage;
+      const int stage = use_stage;
       if (!dead && !mbar_wait(&full[warp][stage], use_phase)) {
-        // stay in step with the group's barriers; the results are lost
+        // go on to the block's barrier; the results are lost
         dead = true;
         if (lane == 0) atomicAdd(&b2k_tu_timeouts, 1u);
       }
@@ -539,63 +527,48 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * w4_war
       const unsigned char* st = ring + stage * STAGE;
 #pragma unroll
       for (int i = 0; i < SBK; ++i) {
-        if (SBK > 1 && k + i >= use.end) break;
-        uint4 wa[RT], wb[RT];
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          const unsigned char* p = st + (t * SBK + i) * 1024 + c * 16;
-          wa[t] = *reinterpret_cast<const uint4*>(p + row_a * 64);
-          wb[t] = *reinterpret_cast<const uint4*>(p + row_b * 64);
-        }
-        float acc[RT][NT][4];
+        if (k + i >= use.end) break;
+        const uint4 wa = *reinterpret_cast<const uint4*>(st + i * 1024 + row_a * 64 + c * 16);
+        const uint4 wb = *reinterpret_cast<const uint4*>(st + i * 1024 + row_b * 64 + c * 16);
+        float acc[NT][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+          const uint32_t w0 = j == 0 ? wa.x : j == 1 ? wa.y : j == 2 ? wa.z : wa.w;
+          const uint32_t w1 = j == 0 ? wb.x : j == 1 ? wb.y : j == 2 ? wb.z : wb.w;
+          const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const uint4 b = *reinterpret_cast<const uint4*>(xat[nt] + (4 * (k + i) + j) * xstep[nt]);
-#pragma unroll
-            for (int t = 0; t < RT; ++t) {
-              const uint32_t w0 = j == 0 ? wa[t].x : j == 1 ? wa[t].y : j == 2 ? wa[t].z : wa[t].w;
-              const uint32_t w1 = j == 0 ? wb[t].x : j == 1 ? wb[t].y : j == 2 ? wb[t].z : wb[t].w;
-              const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
-              if (j * 32 % G == 0)
-                w4_mma_first(acc[t][nt], w0 & 0x000f000fu, w1 & 0x000f000fu, v0 & 0x000f000fu,
-                             v1 & 0x000f000fu, b.x, b.y);
-              else
-                w4_mma(acc[t][nt], w0 & 0x000f000fu, w1 & 0x000f000fu, v0 & 0x000f000fu,
-                       v1 & 0x000f000fu, b.x, b.y);
-              w4_mma(acc[t][nt], w0 & 0x00f000f0u, w1 & 0x00f000f0u, v0 & 0x00f000f0u,
-                     v1 & 0x00f000f0u, b.z, b.w);
-            }
+            const uint4 b = *reinterpret_cast<const uint4*>(smem + xat[nt] + (4 * (k + i) + j) * xstep[nt]);
+            if (j * 32 % G == 0)
+              w4_mma_first(acc[nt], w0 & 0x000f000fu, w1 & 0x000f000fu, v0 & 0x000f000fu,
+                           v1 & 0x000f000fu, b.x, b.y);
+            else
+              w4_mma(acc[nt], w0 & 0x000f000fu, w1 & 0x000f000fu, v0 & 0x000f000fu,
+                     v1 & 0x000f000fu, b.x, b.y);
+            w4_mma(acc[nt], w0 & 0x00f000f0u, w1 & 0x00f000f0u, v0 & 0x00f000f0u,
+                   v1 & 0x00f000f0u, b.z, b.w);
           }
           if ((j + 1) * 32 % G == 0) {
             const int gi = j * 32 / G;
+            // (sum, scale) of columns 2c, 2c + 1 of x; scales and zeros of rows 2r, 2r + 1
             const float4* gp = reinterpret_cast<const float4*>(gsm + ((k + i) * GS + gi) * (8 * NT) + 2 * c);
-            float4 g4[NT];  // (sum, scale) of columns 2c, 2c + 1
+            const uint32_t* sp = reinterpret_cast<const uint32_t*>(st + 2048 + (i * GS + gi) * 32) + r;
+            auto two = [&](uint32_t bits) {
+              bits = __byte_perm(bits, 0, swap);
+              if constexpr (!BF) return __half22float2(*reinterpret_cast<const __half2*>(&bits));
+              else return f2(__uint_as_float(bits << 16), __uint_as_float(bits & 0xffff0000u));
+            };
+            const float2 z = zeros ? two(sp[SBK * GS * 8]) : f2s(8.0f);
+            // 2^10: 2^24 of the integers' unit, 2^-14 of x's
+            const float2 s = mul2(two(*sp), f2s(1024.0f));
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) g4[nt] = gp[nt * 4];
-#pragma unroll
-            for (int t = 0; t < RT; ++t) {
-              // rows 2r, 2r + 1 of the tile
-              const uint32_t* sp = reinterpret_cast<const uint32_t*>(
-                  st + 2048 + ((t * SBK + i) * GS + gi) * 32) + r;
-              auto two = [&](uint32_t bits) {
-                bits = __byte_perm(bits, 0, swap);
-                if constexpr (!BF) return __half22float2(*reinterpret_cast<const __half2*>(&bits));
-                else return f2(__uint_as_float(bits << 16), __uint_as_float(bits & 0xffff0000u));
-              };
-              const float2 z = zeros ? two(sp[2 * GS * 8]) : f2s(8.0f);
-              // 2^10: 2^24 of the integers' unit, 2^-14 of x's
-              const float2 s = mul2(two(*sp), f2s(1024.0f));
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                const float* q = acc[t][nt];
-                const float4 g = g4[nt];
-                y[t][nt][0] = fmaf(fmaf(-z.x, g.x, q[0]) * s.x, g.y, y[t][nt][0]);
-                y[t][nt][1] = fmaf(fmaf(-z.x, g.z, q[1]) * s.x, g.w, y[t][nt][1]);
-                y[t][nt][2] = fmaf(fmaf(-z.y, g.x, q[2]) * s.y, g.y, y[t][nt][2]);
-                y[t][nt][3] = fmaf(fmaf(-z.y, g.z, q[3]) * s.y, g.w, y[t][nt][3]);
-              }
+            for (int nt = 0; nt < NT; ++nt) {
+              const float* q = acc[nt];
+              const float4 g = gp[nt * 4];
+              y[nt][0] = fmaf(fmaf(-z.x, g.x, q[0]) * s.x, g.y, y[nt][0]);
+              y[nt][1] = fmaf(fmaf(-z.x, g.z, q[1]) * s.x, g.w, y[nt][1]);
+              y[nt][2] = fmaf(fmaf(-z.y, g.x, q[2]) * s.y, g.y, y[nt][2]);
+              y[nt][3] = fmaf(fmaf(-z.y, g.z, q[3]) * s.y, g.w, y[nt][3]);
             }
           }
         }
@@ -610,20 +583,16 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * w4_war
     if (!ends) {
       tail_item = use.item - 1;
 #pragma unroll
-      for (int t = 0; t < RT; ++t)
-#pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) tail[t][nt][e] = y[t][nt][e];
+          for (int e = 0; e < 4; ++e) tail[nt][e] = y[nt][e];
     } else {
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int64_t n = (item * RT + t) * 16 + (h ? row_b : row_a);
-            const float v0 = y[t][nt][2 * h], v1 = y[t][nt][2 * h + 1];
+            const int64_t n = item * 16 + (h ? row_b : row_a);
+            const float v0 = y[nt][2 * h], v1 = y[nt][2 * h + 1];
             const int col = nt * 8 + 2 * c;
             if (f32) {
               if (col < C) store(col >> 1, n, fmaf(v1, kLow, v0));
@@ -634,11 +603,9 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * w4_war
           }
     }
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[t][nt][e] = 0.0f;
+        for (int e = 0; e < 4; ++e) y[nt][e] = 0.0f;
   }
   if (dead)  // nothing may land where the parts go
     for (used -= used > 0; used < issued; ++used)
@@ -646,23 +613,21 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * w4_war
 
   // ---- items that span warps: their parts, in the warps' drained rings ----------
   if (kn == 0) {  // no columns at all
-    for (int64_t i = tid; i < (int64_t)n_items * RT * 16 * rows; i += blockDim.x)
-      store((int)(i % rows), i0 * RT * 16 + i / rows, 0.0f);
+    for (int64_t i = tid; i < (int64_t)n_items * 16 * rows; i += blockDim.x)
+      store((int)(i % rows), i0 * 16 + i / rows, 0.0f);
     return;
   }
-  constexpr int PER = RT * 16 * 8 * NT;
+  constexpr int PER = 16 * 8 * NT;
   const bool has_tail = tail_item >= 0;
   __syncwarp();
-  float* mine = reinterpret_cast<float*>(ring);  // [head, tail][column][RT * 16 rows]
-#pragma unroll
-  for (int t = 0; t < RT; ++t)
+  float* mine = reinterpret_cast<float*>(ring);  // [head, tail][column][16 rows]
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int at = (nt * 8 + 2 * c + (e & 1)) * RT * 16 + t * 16 + (e >> 1 ? row_b : row_a);
-        mine[at] = y[t][nt][e];  // zeros where there is no head
-        if (has_tail) mine[PER + at] = tail[t][nt][e];
+        const int at = (nt * 8 + 2 * c + (e & 1)) * 16 + (e >> 1 ? row_b : row_a);
+        mine[at] = y[nt][e];  // zeros where there is no head
+        if (has_tail) mine[PER + at] = tail[nt][e];
       }
   __syncthreads();
   // this warp's tail, and the heads of the next warps whose runs lie in that item
@@ -671,9 +636,9 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * w4_war
   int last = warp;
 #pragma unroll
   for (int w = 1; w < W; ++w) last += w > warp && run_at(w) < past;
-  for (int i = lane; i < rows * RT * 16; i += 32) {
-    const int m = i / (RT * 16), n16 = i - m * RT * 16;
-    const int c0 = (f32 ? 2 * m : m) * RT * 16 + n16, c1 = f32 ? c0 + RT * 16 : c0;
+  for (int i = lane; i < rows * 16; i += 32) {
+    const int m = i >> 4, n16 = i & 15;
+    const int c0 = (f32 ? 2 * m : m) * 16 + n16, c1 = f32 ? c0 + 16 : c0;
     float v = mine[PER + c0], low = mine[PER + c1];
     const float* from = reinterpret_cast<const float*>(smem);
 #pragma unroll 4
@@ -681,7 +646,7 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * w4_war
       v += from[w * (S * STAGE / 4) + c0];
       low += from[w * (S * STAGE / 4) + c1];
     }
-    store(m, (i0 + tail_item) * RT * 16 + n16, f32 ? fmaf(low, kLow, v) : v);
+    store(m, (i0 + tail_item) * 16 + n16, f32 ? fmaf(low, kLow, v) : v);
   }
 }
 
@@ -700,13 +665,12 @@ template <typename T> __global__ void __launch_bounds__(256) w4_sum_kernel(const
 }
 
 // How a product is split.  One block per SM, its warps' rings as deep as shared
-// memory allows beside x (kW4Stages stages at most, and two parts of an item at
-// least); K is split over blocks where x does not fit beside that.  x is
+// memory allows beside x (2 to kW4Stages stages); K is split over blocks where x does not fit beside that.  x is
 // prepared once by a kernel of its own where every block's own preparation
 // would take it more than kW4Own eights of columns per thread.
 constexpr int kW4Own = 4;
 struct W4Plan {
-  int nt, rows, warps, stages, kslice, slices, grid_x, grid_y;
+  int nt, rows, stages, kslice, slices, grid_x, grid_y;
   bool prepare;
   int64_t smem, image, bytes, each, more;
 };
@@ -718,29 +682,27 @@ static W4Plan w4_plan(int64_t M, int64_t N, int64_t K, int group, bool f32) {
   p.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
   p.rows = (int)(M < 8 * p.nt / per ? M : 8 * p.nt / per);
   p.grid_y = (int)((M + p.rows - 1) / p.rows);
-  p.warps = w4_warps(p.nt);
-  const int least = p.nt == 4 ? 4 : 2;  // 2 PER floats fit these stages
+  const int least = 2;  // 2 PER floats fit these stages
   auto need = [&](int64_t kslice, int stages) {
     return w4_x_bytes(kslice, p.rows * per) + w4_g_bytes(kslice, gs, p.nt) +
-           (int64_t)p.warps * stages * w4_stage(gs);
+           (int64_t)kW4Warps * stages * w4_stage(gs) + 16;
   };
   p.slices = 1;
   p.kslice = (int)(KT > 0 ? KT : 1);
-  while (need(p.kslice, least) > kW4Smem) {
+  while (need(p.kslice, 2) > kW4Smem) {
     ++p.slices;
     p.kslice = (int)((KT + p.slices - 1) / p.slices);
   }
   p.slices = KT > 0 ? (int)((KT + p.kslice - 1) / p.kslice) : 1;
   p.stages = kW4Stages;
   while (need(p.kslice, p.stages) > kW4Smem) --p.stages;
-  p.prepare = (int64_t)p.rows * p.kslice * 16 > kW4Own * 32 * p.warps;
+  p.prepare = (int64_t)p.rows * p.kslice * 16 > kW4Own * 32 * kW4Warps;
   p.smem = need(p.kslice, p.stages);
-  const int64_t items = (tiles + w4_rt(p.nt) - 1) / w4_rt(p.nt);
   int64_t slots = (int64_t)sm_count() / (p.slices * p.grid_y);
   if (slots < 1) slots = 1;
-  p.grid_x = (int)(items < slots ? items : slots);
-  p.each = items / p.grid_x;
-  p.more = items % p.grid_x;
+  p.grid_x = (int)(tiles < slots ? tiles : slots);
+  p.each = tiles / p.grid_x;
+  p.more = tiles % p.grid_x;
   p.image = p.prepare ? p.grid_y * w4_image_bytes(KT, p.rows * per, gs, p.nt) : 0;
   p.bytes = p.image + (p.slices > 1 ? (int64_t)p.slices * M * N * 4 : 0);
   return p;
@@ -753,7 +715,7 @@ template <int NT, int GS, bool BF> static void w4_launch(const W4Args& a, const 
   }
   auto kern = w4_kernel<NT, GS, BF>;
   allow_max_dynamic_smem(kern);
-  launch_pdl(kern, dim3(p.grid_x, p.grid_y, p.slices), dim3(32 * p.warps), (size_t)p.smem, st, a);
+  launch_pdl(kern, dim3(p.grid_x, p.grid_y, p.slices), dim3(32 * kW4Warps), (size_t)p.smem, st, a);
 }
 
 template <int NT, bool BF> static void w4_dispatch(const W4Args& a, const W4Plan& p, cudaStream_t st) {
