@@ -530,7 +530,10 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * kW4War
         if (k + i >= use.end) break;
         const uint4 wa = *reinterpret_cast<const uint4*>(st + i * 1024 + row_a * 64 + c * 16);
         const uint4 wb = *reinterpret_cast<const uint4*>(st + i * 1024 + row_b * 64 + c * 16);
-        float acc[NT][4];
+        // two sums for 8 columns (even and odd nibbles), so that half as many
+        // products wait for one another
+        constexpr int CH = NT == 1 ? 2 : 1;
+        float acc[CH][NT][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t w0 = j == 0 ? wa.x : j == 1 ? wa.y : j == 2 ? wa.z : wa.w;
@@ -540,13 +543,17 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * kW4War
           for (int nt = 0; nt < NT; ++nt) {
             const uint4 b = *reinterpret_cast<const uint4*>(smem + xat[nt] + (4 * (k + i) + j) * xstep[nt]);
             if (j * 32 % G == 0)
-              w4_mma_first(acc[nt], w0 & 0x000f000fu, w1 & 0x000f000fu, v0 & 0x000f000fu,
+              w4_mma_first(acc[0][nt], w0 & 0x000f000fu, w1 & 0x000f000fu, v0 & 0x000f000fu,
                            v1 & 0x000f000fu, b.x, b.y);
             else
-              w4_mma(acc[nt], w0 & 0x000f000fu, w1 & 0x000f000fu, v0 & 0x000f000fu,
+              w4_mma(acc[0][nt], w0 & 0x000f000fu, w1 & 0x000f000fu, v0 & 0x000f000fu,
                      v1 & 0x000f000fu, b.x, b.y);
-            w4_mma(acc[nt], w0 & 0x00f000f0u, w1 & 0x00f000f0u, v0 & 0x00f000f0u,
-                   v1 & 0x00f000f0u, b.z, b.w);
+            if (CH == 2 && j * 32 % G == 0)
+              w4_mma_first(acc[CH - 1][nt], w0 & 0x00f000f0u, w1 & 0x00f000f0u, v0 & 0x00f000f0u,
+                           v1 & 0x00f000f0u, b.z, b.w);
+            else
+              w4_mma(acc[CH - 1][nt], w0 & 0x00f000f0u, w1 & 0x00f000f0u, v0 & 0x00f000f0u,
+                     v1 & 0x00f000f0u, b.z, b.w);
           }
           if ((j + 1) * 32 % G == 0) {
             const int gi = j * 32 / G;
@@ -563,7 +570,9 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * kW4War
             const float2 s = mul2(two(*sp), f2s(1024.0f));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              const float* q = acc[nt];
+              float q[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) q[e] = CH == 2 ? acc[0][nt][e] + acc[CH - 1][nt][e] : acc[0][nt][e];
               const float4 g = gp[nt * 4];
               y[nt][0] = fmaf(fmaf(-z.x, g.x, q[0]) * s.x, g.y, y[nt][0]);
               y[nt][1] = fmaf(fmaf(-z.x, g.z, q[1]) * s.x, g.w, y[nt][1]);
@@ -682,7 +691,6 @@ static W4Plan w4_plan(int64_t M, int64_t N, int64_t K, int group, bool f32) {
   p.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
   p.rows = (int)(M < 8 * p.nt / per ? M : 8 * p.nt / per);
   p.grid_y = (int)((M + p.rows - 1) / p.rows);
-  const int least = 2;  // 2 PER floats fit these stages
   auto need = [&](int64_t kslice, int stages) {
     return w4_x_bytes(kslice, p.rows * per) + w4_g_bytes(kslice, gs, p.nt) +
            (int64_t)kW4Warps * stages * w4_stage(gs) + 16;
