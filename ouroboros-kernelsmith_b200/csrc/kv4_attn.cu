@@ -239,7 +239,7 @@ __device__ __forceinline__ void attn_step(const Kv4AttnArgs& a, AttnWalk& k) {
   }
 }
 
-template <int D, int GRP, int NT, int T>
+template <int D, int GRP, int NT, int T, bool SPLIT>
 __global__ void __launch_bounds__(32 * kAttnWarps, attn_cps(D, NT))
 kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
   using X = AttnShape<D, GRP, NT, T>;
@@ -319,9 +319,10 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
   bool timeout = false;
 
   // ---- the ring: the walk `get` runs ahead of `use` by up to S tiles ---------
-  // A tile lies within a page.  get_src: its bytes, for as long as the page (or
-  // the part) lasts, up to tile get_stop; a page is looked up one call before
-  // it is needed.
+  // Where pages hold tiles whole, get_src is a tile's bytes for as long as the
+  // page (or the part) lasts, up to tile get_stop; a page is looked up one call
+  // before it is needed.  Else (SPLIT) lanes 0 and 1 look up and copy 16 tokens
+  // each (two copies by one lane: 75 against 56 us at 32 x 8192, D 64, P 16).
   int get_stop = 0, get_end = 0, get_pid = 0, get_at = 0, get_stage = 0;
   const int32_t* get_page = nullptr;
   const unsigned char* get_src = nullptr;
@@ -329,38 +330,66 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
   bool bad = false, my_first = false, my_last = false;
   uint32_t bad_stages = 0;  // stages of tokens whose page is outside the pool
   const int64_t head_bytes = (int64_t)(a.c.P >> 4) * MB;
+  auto look_up = [&](int tok) {
+    const int pi = a.dP.div(tok);
+    get_at = tok - pi * a.c.P;
+    get_pid = tok < get_end ? get_page[pi] : -1;
+  };
   auto open = [&]() {  // the next part's first tile
     getting = attn_next<D, NT, T>(a, get);
     if (getting) {
-      const int b = a.dRT.div(get.entry), tok = get.t * T, pi = a.dP.div(tok);
+      const int b = a.dRT.div(get.entry), tok = get.t * T;
       bool over;
       get_end = attn_end<D, NT>(a, attn_len(a, b, over), get.entry - b * a.RT);
-      get_page = a.table + b * a.width + pi;
-      get_pid = get_end > 0 ? *get_page : -1;
-      get_at = tok - pi * a.c.P;
-      get_stop = min(get.t1, get.t + (a.c.P - get_at) / T);
-      get_fresh = true;
+      get_page = a.table + b * a.width;
+      if constexpr (SPLIT) {
+        look_up(tok + 16 * (lane & 1));
+        get_stop = get.t1;
+      } else {
+        const int pi = a.dP.div(tok);
+        get_page += pi;
+        get_pid = get_end > 0 ? *get_page : -1;
+        get_at = tok - pi * a.c.P;
+        get_stop = min(get.t1, get.t + (a.c.P - get_at) / T);
+        get_fresh = true;
+      }
     }
   };
+  auto micro = [&](int pid, int at) {
+    return a.c.data + ((int64_t)pid * a.c.Hk + get.head) * head_bytes + (at >> 4) * MB;
+  };
   auto issue = [&]() {
-    if (get_fresh) {
-      get_fresh = false;
-      get_ok = (uint32_t)get_pid < (uint32_t)a.c.pages;
-      get_src = a.c.data + ((int64_t)get_pid * a.c.Hk + get.head) * head_bytes + (get_at >> 4) * MB;
-    }
-    if (lane == 0) {
-      uint64_t* bar = &full[warp][get_stage];
+    uint64_t* bar = &full[warp][get_stage];
+    unsigned char* dst = ring + get_stage * X::STAGE;
+    bool miss;
+    if constexpr (SPLIT) {
+      const bool want = lane < 2 && get.t * T + 16 * lane < get_end;
+      const bool ok = want && (uint32_t)get_pid < (uint32_t)a.c.pages;
+      const uint32_t n = __popc(__ballot_sync(0xffffffffu, ok));
+      miss = __any_sync(0xffffffffu, want && !ok);
       fence_proxy_async();
-      mbar_arrive_expect_tx(bar, get_ok ? X::STAGE : 0);
-      if (get_ok) bulk_g2s(ring + get_stage * X::STAGE, get_src, X::STAGE, bar);
+      if (lane == 0) mbar_arrive_expect_tx(bar, n * MB);
+      __syncwarp();
+      if (ok) bulk_g2s(dst + lane * MB, micro(get_pid, get_at), MB, bar);
+    } else {
+      if (get_fresh) {
+        get_fresh = false;
+        get_ok = (uint32_t)get_pid < (uint32_t)a.c.pages;
+        get_src = micro(get_pid, get_at);
+      }
+      miss = !get_ok && get_end > 0;
+      if (lane == 0) {
+        fence_proxy_async();
+        mbar_arrive_expect_tx(bar, get_ok ? X::STAGE : 0);
+        if (get_ok) bulk_g2s(dst, get_src, X::STAGE, bar);
+      }
+      get_src += X::STAGE;
     }
-    get_src += X::STAGE;
-    if (!get_ok || bad_stages)
-      bad_stages = (bad_stages & ~(1u << get_stage)) | ((uint32_t)(!get_ok && get_end > 0) << get_stage);
+    if (miss || bad_stages) bad_stages = (bad_stages & ~(1u << get_stage)) | ((uint32_t)miss << get_stage);
     if (++get_stage == S) get_stage = 0;
     ++issued;
     if (++get.t == get_stop) {
-      if (get.t == get.t1) {
+      if (SPLIT || get.t == get.t1) {
         attn_step(a, get);
         open();
       } else {
@@ -369,6 +398,8 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
         get_stop = min(get.t1, get_stop + a.c.P / T);
         get_fresh = true;
       }
+    } else if constexpr (SPLIT) {
+      look_up(get.t * T + 16 * (lane & 1));
     }
   };
   open();
@@ -846,13 +877,22 @@ __global__ void __launch_bounds__(D / 4 * kMergeSlices) kv4_attn_merge_kernel(
       L = fmaf(p.y, f, L);
     }
     __syncthreads();
-#pragma unroll 8
-    for (int i = slice; i < n; i += kMergeSlices) {
-      const float f = weight[i];
-      if (f != 0.0f) {  // a part that holds nothing has no output either
-        const float4 t = *reinterpret_cast<const float4*>(a.part + slot(base + i) * D + 4 * d4);
-        v.x = fmaf(t.x, f, v.x); v.y = fmaf(t.y, f, v.y);
-        v.z = fmaf(t.z, f, v.z); v.w = fmaf(t.w, f, v.w);
+    for (int i = slice; i < n; i += 8 * kMergeSlices) {
+      // eight loads together; a part that holds nothing has no output either
+      float4 t[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int k = i + j * kMergeSlices;
+        t[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (k < n && weight[k] != 0.0f)
+          t[j] = *reinterpret_cast<const float4*>(a.part + slot(base + k) * D + 4 * d4);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int k = i + j * kMergeSlices;
+        const float f = k < n ? weight[k] : 0.0f;
+        v.x = fmaf(t[j].x, f, v.x); v.y = fmaf(t[j].y, f, v.y);
+        v.z = fmaf(t[j].z, f, v.z); v.w = fmaf(t[j].w, f, v.w);
       }
     }
   }
@@ -874,6 +914,58 @@ __global__ void __launch_bounds__(D / 4 * kMergeSlices) kv4_attn_merge_kernel(
   *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + (((int64_t)b * a.Sq + i) * a.H + hq) * D +
                             4 * d4) = attn_pack4(v, attn_inverse(L), a.bf16);
   if (a.lse && d4 == 0) a.lse[((int64_t)b * a.H + hq) * a.Sq + i] = attn_lse(M, L);
+}
+
+// The same for many segments, of few parts each: every thread merges four
+// dimensions of one row by itself, a block holds 1024 / D rows.
+template <int D, int NT>
+__global__ void __launch_bounds__(256) kv4_attn_merge_few_kernel(const __grid_constant__ Kv4AttnArgs a) {
+  constexpr int ROWS = attn_rows(NT);
+  griddep_launch_dependents();
+  griddep_wait();
+  const int seg = blockIdx.x, row = blockIdx.y * (1024 / D) + threadIdx.x / (D / 4);
+  const int d = threadIdx.x % (D / 4) * 4;
+  const int2 span = a.spans[seg];
+  if (span.x == span.y) return;
+  const int entry = a.dHk.div(seg), b = a.dRT.div(entry), head = seg - entry * a.c.Hk;
+  const int rr = (entry - b * a.RT) * ROWS + row, parts = span.y - span.x + 1;
+  if (row >= ROWS || rr >= (int)(a.Sq * a.G)) return;
+  auto slot = [&](int i) { return (2 * (int64_t)(span.x + i) + (i == 0 ? 1 : 0)) * ROWS + row; };
+  float M = -INFINITY, L = 0.0f;
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int base = 0; base < parts; base += 4) {
+    // four parts' loads together, the sums so far moved to their maximum
+    float2 p[4];
+    float4 t[4];
+    float Mn = M;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      p[j] = base + j < parts ? *attn_ml(a, slot(base + j), ROWS * D) : make_float2(-INFINITY, 0.0f);
+      Mn = fmaxf(Mn, p[j].x);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // a part that holds nothing has no output either
+      t[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (!(p[j].x == -INFINITY && p[j].y == 0.0f))
+        t[j] = *reinterpret_cast<const float4*>(a.part + slot(base + j) * D + d);
+    }
+    const float f0 = attn_weight(M, L, Mn);
+    L *= f0;
+    v.x *= f0; v.y *= f0; v.z *= f0; v.w *= f0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float f = attn_weight(p[j].x, p[j].y, Mn);
+      L = fmaf(p[j].y, f, L);
+      v.x = fmaf(t[j].x, f, v.x); v.y = fmaf(t[j].y, f, v.y);
+      v.z = fmaf(t[j].z, f, v.z); v.w = fmaf(t[j].w, f, v.w);
+    }
+    M = Mn;
+  }
+  const int i = a.dG.div(rr), hq = head * a.G + (rr - i * a.G);
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + (((int64_t)b * a.Sq + i) * a.H + hq) * D + d) =
+      attn_pack4(v, attn_inverse(L), a.bf16);
+  if (a.lse && d == 0) a.lse[((int64_t)b * a.H + hq) * a.Sq + i] = attn_lse(M, L);
 }
 
 // columns of the products, in eights: the fewest that hold the rows, up to
@@ -902,9 +994,9 @@ static AttnPlan attn_plan(int64_t B, int64_t Sq, int64_t H, int64_t Hk, int64_t 
   return p;
 }
 
-template <int D, int GRP, int NT, int T>
+template <int D, int GRP, int NT, int T, bool SPLIT>
 static int attn_launch(const Kv4AttnArgs& a, const AttnPlan& p, cudaStream_t st) {
-  auto kern = kv4_attn_kernel<D, GRP, NT, T>;
+  auto kern = kv4_attn_kernel<D, GRP, NT, T, SPLIT>;
   static bool done[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -914,20 +1006,29 @@ static int attn_launch(const Kv4AttnArgs& a, const AttnPlan& p, cudaStream_t st)
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
   launch_pdl(kern, dim3(p.blocks), dim3(32 * kAttnWarps), AttnShape<D, GRP, NT, T>::SMEM, st, a);
-  launch_pdl(kv4_attn_merge_kernel<D, NT>, dim3((unsigned)p.segs, 8 * NT), dim3(D / 4 * kMergeSlices), 0,
-             st, a);
+  // a segment has about warps / segments parts
+  const unsigned rows = (unsigned)(a.Sq * a.G < 8 * NT ? a.Sq * a.G : 8 * NT);
+  if (p.segs >= 2 * sm_count())
+    launch_pdl(kv4_attn_merge_few_kernel<D, NT>, dim3((unsigned)p.segs, (rows + 1024 / D - 1) / (1024 / D)),
+               dim3(256), 0, st, a);
+  else
+    launch_pdl(kv4_attn_merge_kernel<D, NT>, dim3((unsigned)p.segs, rows), dim3(D / 4 * kMergeSlices), 0,
+               st, a);
   return check_launch("b2k_kv4_attention");
 }
 
-// Tiles of 32 tokens where pages hold them whole and registers their scores
-// (NT T / 8 per thread beside the output's NT D / 4), else of 16: 83 against
-// 94 us at 16 sequences of 16384 tokens, D 128.
+// Tiles of 32 tokens where registers hold their scores (NT T / 8 per thread
+// beside the output's NT D / 4), else of 16: 83 against 94 us at 16 sequences of
+// 16384 tokens, D 128.  Pages that are no multiple of 32 tokens take two copies
+// per tile.
 template <int D, int GRP, int NT>
 static int attn_tokens(const Kv4AttnArgs& a, const AttnPlan& p, cudaStream_t st) {
   if constexpr (D < 256 && NT * D <= 256) {
-    if (a.c.P % 32 == 0) return attn_launch<D, GRP, NT, 32>(a, p, st);
+    if (a.c.P % 32 == 0) return attn_launch<D, GRP, NT, 32, false>(a, p, st);
+    return attn_launch<D, GRP, NT, 32, true>(a, p, st);
+  } else {
+    return attn_launch<D, GRP, NT, 16, false>(a, p, st);
   }
-  return attn_launch<D, GRP, NT, 16>(a, p, st);
 }
 
 template <int D, int GRP>
