@@ -28,7 +28,7 @@
 //
 // Work is split by tiles of tokens, not by sequences: all (sequence, row
 // tile, head) segments are laid end to end and every warp takes an equal run
-// of tiles (a segment counts kAttnLead more for its own costs), found on the
+// of tiles (a segment counts some more for its own costs), found on the
 // device from the lengths, which the host does not know; so ragged batches and
 // single long sequences fill the GPU alike.  Warps are independent: each has
 // its own ring of bulk copies, which runs ahead across segments, and writes
@@ -51,8 +51,6 @@ constexpr int kAttnWarps = 4;
 constexpr int kAttnStages = 3;
 constexpr float kPScale = 10.0f;  // probabilities are held times 2^10
 constexpr float kPSlack = 4.0f;   // ... and below 2^(10 + 4) until the maximum is moved
-constexpr int kAttnLead = 2;      // a segment's fixed costs, in tiles
-constexpr int kAttnLeast = 2;     // tiles of a run beside them
 
 // 64-bit division that takes the short way for what fits 32 bits
 __device__ __forceinline__ int64_t wide_div(int64_t n, int64_t d) {
@@ -211,6 +209,7 @@ __device__ __forceinline__ float2* attn_ml(const Kv4AttnArgs& a, int64_t slot_ro
 // (entry, head), which has n.
 struct AttnWalk {
   int entry, head, n, pos, left;  // pos: units of the segment already taken
+  int lead;                       // a segment's fixed costs, in units of a tile
   int t, t1;
 };
 // on to the next part that has tiles
@@ -218,9 +217,9 @@ template <int D, int NT, int T>
 __device__ __forceinline__ bool attn_next(const Kv4AttnArgs& a, AttnWalk& k) {
   while (k.left > 0) {
     if (k.n == 0) k.n = attn_tiles<D, NT, T>(a, k.entry);
-    const int take = min(k.left, k.n + kAttnLead - k.pos);
-    k.t = max(k.pos - kAttnLead, 0);
-    k.t1 = max(k.pos + take - kAttnLead, 0);
+    const int take = min(k.left, k.n + k.lead - k.pos);
+    k.t = max(k.pos - k.lead, 0);
+    k.t1 = max(k.pos + take - k.lead, 0);
     k.left -= take;
     k.pos += take;
     if (k.t1 > k.t) return true;
@@ -230,7 +229,7 @@ __device__ __forceinline__ bool attn_next(const Kv4AttnArgs& a, AttnWalk& k) {
 }
 // past a finished part
 __device__ __forceinline__ void attn_step(const Kv4AttnArgs& a, AttnWalk& k) {
-  if (k.pos < k.n + kAttnLead) return;  // the run ends within the segment
+  if (k.pos < k.n + k.lead) return;  // the run ends within the segment
   k.pos = 0;
   if (++k.head == a.c.Hk) {
     k.head = 0;
@@ -264,20 +263,24 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
   const int chunk = (entries + 31) / 32;
   const int e0 = min(entries, lane * chunk), e1 = min(entries, e0 + chunk);
   int64_t mine = 0;
-  for (int e = e0; e < e1; ++e) mine += attn_tiles<D, NT, T>(a, e) + kAttnLead;
+  for (int e = e0; e < e1; ++e) mine += attn_tiles<D, NT, T>(a, e);
   int64_t before = mine;
 #pragma unroll
   for (int x = 1; x < 32; x <<= 1) {
     const int64_t t = __shfl_up_sync(0xffffffffu, before, x);
     if (lane >= x) before += t;
   }
-  const int64_t total = __shfl_sync(0xffffffffu, before, 31) * a.c.Hk;
-  mine *= a.c.Hk;
-  before = before * a.c.Hk - mine;
-  // a run is a segment's lead and kAttnLeast tiles at least; the first `more`
-  // runs are one unit longer than `each`
-  const int64_t runs = min((int64_t)gridDim.x * kAttnWarps,
-                           wide_div(total + kAttnLead + kAttnLeast - 1, kAttnLead + kAttnLeast));
+  const int64_t tiles = __shfl_sync(0xffffffffu, before, 31) * a.c.Hk, warps = (int64_t)gridDim.x * kAttnWarps;
+  // What a segment costs beside its tiles (its queries, its results) and the
+  // least units of a run: with many tiles per warp 4 and with few 2 measured
+  // best (64 ragged sequences 50.5 against 54.5 us, 16 x 5 tokens 19.7 against
+  // 17.6, 1 x 1021 13.1 against 11.1).
+  const int lead = tiles >= 8 * warps ? 4 : 2, least = lead + 1;
+  before = (before - mine + (int64_t)e0 * lead) * a.c.Hk;
+  mine = (mine + (int64_t)(e1 - e0) * lead) * a.c.Hk;
+  const int64_t total = tiles + (int64_t)entries * a.c.Hk * lead;
+  // the first `more` runs are one unit longer than `each`
+  const int64_t runs = min(warps, wide_div(total + least - 1, least));
   const int64_t each = wide_div(total, runs), more = total - each * runs;
   auto run_at = [&](int64_t i) { return i * each + min(i, more); };
   auto run_of = [&](int64_t u) {
@@ -286,6 +289,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
   const int64_t run0 = (int64_t)blockIdx.x * kAttnWarps, run = run0 + warp;
   if (run0 >= runs) return;
   AttnWalk use = {};
+  use.lead = lead;
   bool one_segment = false;  // of all the block's runs
   const int64_t u1 = run_at(min(run + 1, runs));
   if (run < runs) {
@@ -296,7 +300,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
     if (here)
       for (;; ++e) {
         n = attn_tiles<D, NT, T>(a, e);
-        const int64_t all = (int64_t)(n + kAttnLead) * a.c.Hk;
+        const int64_t all = (int64_t)(n + lead) * a.c.Hk;
         if (at < all) break;
         at -= all;
       }
@@ -304,12 +308,12 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
     use.entry = __shfl_sync(0xffffffffu, e, src);
     use.n = __shfl_sync(0xffffffffu, n, src);
     at = __shfl_sync(0xffffffffu, at, src);
-    use.head = (int)wide_div(at, use.n + kAttnLead);
-    use.pos = (int)(at - (int64_t)use.head * (use.n + kAttnLead));
+    use.head = (int)wide_div(at, use.n + lead);
+    use.pos = (int)(at - (int64_t)use.head * (use.n + lead));
     use.left = (int)(u1 - u0);
     const int64_t base = u0 - use.pos;  // of the segment
     one_segment = base <= run_at(run0) &&
-                  run_at(min(run0 + kAttnWarps, runs)) <= base + use.n + kAttnLead;
+                  run_at(min(run0 + kAttnWarps, runs)) <= base + use.n + lead;
   }
   // the warps past the last run join the merge of the others
   one_segment = __syncthreads_or(one_segment) != 0;
@@ -720,7 +724,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
     const int64_t seg = (int64_t)use.entry * a.c.Hk + head;
     if (t0 == 0 && lane == 0) {
       // runs that hold the segment's first and last tile
-      const int64_t past = u1 - use.left - use.pos + use.n + kAttnLead;
+      const int64_t past = u1 - use.left - use.pos + use.n + lead;
       a.spans[seg] = make_int2((int)run, whole ? (int)run : (int)run_of(past - 1));
     }
     if (one_segment) {  // the only part: the block's warps meet below
