@@ -20,13 +20,28 @@ import math
 import torch
 
 from . import _lib as L
-from .ops import _DT, _cuda, _dev, _dtype_id, _p, _rows, _same_dtype, _vec
+from .ops import _DT, _cuda, _dev, _dtype_id, _p, _raw_stream, _rows, _same_dtype, _vec
 
 __all__ = ["rmsnorm_quant", "add_rmsnorm_quant", "KVCache4", "kv_cache_write", "kv_cache_read",
            "cache_attention", "W4Weight", "w4_pack", "w4_quantize", "w4_matmul"]
 
 _Q8 = {torch.int8: L.I8, torch.float8_e4m3fn: L.E4M3}
 _DT16 = {torch.float16: L.F16, torch.bfloat16: L.BF16}
+
+
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _call(dev, fn, name, *args):
+    """fn(*args, stream) on dev's current stream, with dev made current; raises
+    B200KError when it fails.  The usual case, dev already current, takes no
+    context manager: these calls are short beside the host's part of them."""
+    if _raw_stream is not None and _device() == dev.index:
+        st = fn(*args, _raw_stream(dev.index))
+    else:
+        with _dev(dev) as stream:
+            st = fn(*args, stream)
+    L.check(st, name)
 
 
 def _dt16(t: torch.dtype, what: str) -> int:
@@ -62,10 +77,8 @@ def _norm_quant(x, residual, w, dtype, group, eps):
     ns = 1 if group is None else (n + group - 1) // group
     q = torch.empty((m, n), dtype=dtype, device=dev)
     scale = torch.empty((m, ns), dtype=torch.float32, device=dev)
-    with _dev(dev) as stream:
-        st = L.lib.b2k_norm_quant(_p(x2), ldx, _p(r2), ldr, _p(w1), _p(h), n, _p(q), n,
-                                  _p(scale), ns, m, n, dt, qt, group or 0, eps, stream)
-    L.check(st, "b2k_norm_quant")
+    _call(dev, L.lib.b2k_norm_quant, "b2k_norm_quant", _p(x2), ldx, _p(r2), ldr, _p(w1), _p(h), n,
+          _p(q), n, _p(scale), ns, m, n, dt, qt, group or 0, eps)
     if x.dim() != 2:
         q = q.view(x.shape)
         scale = scale.view(x.shape[:-1] + (ns,))
@@ -107,7 +120,7 @@ class KVCache4:
     magnitudes above 65408 saturate and a NaN makes its group NaN.  Slot
     t = page * page_size + offset names a token."""
 
-    __slots__ = ("data", "pages", "kv_heads", "page_size", "head_dim", "group")
+    __slots__ = ("data", "pages", "kv_heads", "page_size", "head_dim", "group", "_args", "_sizes")
 
     def __init__(self, data: torch.Tensor, head_dim: int, group: int = 32):
         if head_dim not in (64, 128, 256):
@@ -127,6 +140,8 @@ class KVCache4:
         self.pages, self.kv_heads = data.shape[0], data.shape[1]
         self.page_size = 16 * data.shape[2]
         self.head_dim, self.group = head_dim, group
+        self._args = (data.data_ptr(), self.pages, self.kv_heads, self.page_size, head_dim, group)
+        self._sizes = {}  # workspace bytes of cache_attention by (B, Sq, H)
 
     @classmethod
     def zeros(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, group: int = 32,
@@ -177,11 +192,9 @@ def kv_cache_write(cache: KVCache4, k, v, slots) -> None:
         v = v.contiguous()
     n = k.shape[0]
     s1 = _check_slots(slots, n)
-    with _dev(dev) as stream:
-        st = L.lib.b2k_kv4_write(_p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1),
-                                 _p(s1), n, _p(cache.data), cache.pages, hk, cache.page_size, d,
-                                 cache.group, dt, stream)
-    L.check(st, "b2k_kv4_write")
+    (ldk, hdk, _), (ldv, hdv, _) = k.stride(), v.stride()
+    _call(dev, L.lib.b2k_kv4_write, "b2k_kv4_write", k.data_ptr(), ldk, hdk, v.data_ptr(), ldv, hdv,
+          s1.data_ptr(), n, *cache._args, dt)
 
 
 def kv_cache_read(cache: KVCache4, slots, *, dtype: torch.dtype = torch.bfloat16):
@@ -195,11 +208,8 @@ def kv_cache_read(cache: KVCache4, slots, *, dtype: torch.dtype = torch.bfloat16
     shape = tuple(slots.shape) + (cache.kv_heads, cache.head_dim)
     k = torch.empty(shape, dtype=dtype, device=dev)
     v = torch.empty(shape, dtype=dtype, device=dev)
-    with _dev(dev) as stream:
-        st = L.lib.b2k_kv4_read(_p(cache.data), cache.pages, cache.kv_heads, cache.page_size,
-                                cache.head_dim, cache.group, _p(s1), s1.shape[0], _p(k), _p(v), dt,
-                                stream)
-    L.check(st, "b2k_kv4_read")
+    _call(dev, L.lib.b2k_kv4_read, "b2k_kv4_read", *cache._args, s1.data_ptr(), s1.shape[0],
+          k.data_ptr(), v.data_ptr(), dt)
     return k, v
 
 
@@ -234,15 +244,15 @@ def cache_attention(q, cache: KVCache4, page_table, lengths, *, scale: float | N
     page_table, lengths = page_table.contiguous(), lengths.contiguous()
     o = torch.empty((b, sq, h, d), dtype=q.dtype, device=dev)
     lse = torch.empty((b, h, sq), dtype=torch.float32, device=dev) if return_lse else None
-    nws = L.lib.b2k_kv4_attention_workspace(b, sq, h, hk, d)
-    with _dev(dev) as stream:
-        ws = torch.empty((nws,), dtype=torch.uint8, device=dev) if nws > 0 else None
-        st = L.lib.b2k_kv4_attention(_p(q), q.stride(0), q.stride(1), q.stride(2), _p(o), _p(lse),
-                                     _p(cache.data), cache.pages, hk, cache.page_size, d,
-                                     cache.group, _p(page_table), page_table.shape[1],
-                                     _p(lengths), b, sq, h, d ** -0.5 if scale is None else scale,
-                                     1 if causal else 0, dt, _p(ws), max(nws, 0), stream)
-    L.check(st, "b2k_kv4_attention")
+    nws = cache._sizes.get((b, sq, h))
+    if nws is None:
+        with _dev(dev):
+            nws = L.lib.b2k_kv4_attention_workspace(b, sq, h, hk, d)
+        cache._sizes[(b, sq, h)] = nws
+    ws = torch.empty((nws,), dtype=torch.uint8, device=dev) if nws > 0 else None
+    _call(dev, L.lib.b2k_kv4_attention, "b2k_kv4_attention", q.data_ptr(), *q.stride()[:3], o.data_ptr(),
+          _p(lse), *cache._args, page_table.data_ptr(), page_table.shape[1], lengths.data_ptr(), b, sq, h,
+          d ** -0.5 if scale is None else scale, 1 if causal else 0, dt, _p(ws), nws)
     return (o, lse) if return_lse else o
 
 
@@ -259,7 +269,7 @@ class W4Weight:
     [ceil(n/16), ceil(k/128), 128 / group, 16].  w4_pack and w4_quantize
     make them."""
 
-    __slots__ = ("tiles", "scales", "zeros", "n", "k", "group", "_args")
+    __slots__ = ("tiles", "scales", "zeros", "n", "k", "group", "_args", "_sizes")
 
     def __init__(self, tiles, scales, zeros, n: int, k: int):
         _cuda(tiles, scales, zeros)
@@ -283,6 +293,7 @@ class W4Weight:
         self.tiles, self.scales, self.zeros = tiles, scales, zeros
         self.n, self.k, self.group = n, k, 128 // scales.shape[2]
         self._args = (_p(tiles), _p(scales), _p(zeros), st, self.group)
+        self._sizes = {}  # workspace bytes of w4_matmul by (rows, x's type)
 
 
 def _w4_empty(n, k, group, stype, with_zeros, dev):
@@ -388,11 +399,12 @@ def w4_matmul(x, weight: W4Weight, *, x_scale=None, out_dtype: torch.dtype | Non
     if out_dtype not in _DT:
         raise TypeError(f"b200k: unsupported out_dtype {out_dtype}")
     y = torch.empty((m, n), dtype=out_dtype, device=dev)
-    tiles, scales, zeros, st, _ = weight._args
-    with _dev(dev) as stream:
-        nws = L.lib.b2k_w4_matmul_workspace(m, n, k, group, xt)
-        ws = torch.empty((nws,), dtype=torch.uint8, device=dev) if nws > 0 else None
-        L.check(L.lib.b2k_w4_matmul(_p(x2), ldx, xt, _p(xs), ldxs, xg, tiles, scales, zeros, st,
-                                    group, m, n, k, _p(y), n, _DT[out_dtype], _p(ws), nws, stream),
-                "b2k_w4_matmul")
+    nws = weight._sizes.get((m, xt))
+    if nws is None:
+        with _dev(dev):
+            nws = L.lib.b2k_w4_matmul_workspace(m, n, k, group, xt)
+        weight._sizes[(m, xt)] = nws
+    ws = torch.empty((nws,), dtype=torch.uint8, device=dev) if nws > 0 else None
+    _call(dev, L.lib.b2k_w4_matmul, "b2k_w4_matmul", x2.data_ptr(), ldx, xt, _p(xs), ldxs, xg,
+          *weight._args, m, n, k, y.data_ptr(), n, _DT[out_dtype], _p(ws), nws)
     return y if x.dim() == 2 else y.view(x.shape[:-1] + (n,))
