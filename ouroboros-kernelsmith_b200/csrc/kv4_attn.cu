@@ -23,6 +23,12 @@
 //     wait for the sum: lo + s n is formed in float16 (one rounding, 2^-11) and
 //     meets probabilities in float16 (2^-11), sums in fp32.  Probabilities are
 //     held times 2^10, which keeps small ones out of the subnormals.
+//     With one group for the whole head (g = D) the parameters can go with the
+//     tokens after all: sum_t p_t (lo_t + s_t n_t) = sum_t (p_t s_t) n_t + sum_t
+//     p_t lo_t, the integers again as they are, p s formed in fp32 and rounded
+//     once, the second sum one fp32 number per row (8 x 65536 tokens, D 128, g
+//     128: 112 us instead of 135).  The running maximum is then that of p s, so that these
+//     products use float16's range whatever the values' magnitude.
 //   * The running maximum and sum are fp32, per lane for its own tokens; the
 //     output is rescaled only when a row's maximum has moved by 2^4.
 //
@@ -170,6 +176,7 @@ __device__ __forceinline__ void value_pairs(uint32_t x, __half2 s, __half2 lo, c
 template <int D, int GRP, int NT, int T> struct AttnShape {
   static constexpr int U = T / 16, J = D / 32, NG = D / GRP, ROWS = attn_rows(NT);
   static constexpr int MB = 16 * (D + 8 * NG);           // bytes of a micro block
+  static constexpr bool FOLD = NG == 1;                  // values' parameters with the tokens
   static constexpr int KP = 8 * D, VR = KP + 64 * NG, VP = VR + 8 * D;  // its fields
   static constexpr int STAGE = U * MB;
   static constexpr int MERGE = kAttnWarps * ROWS * D * 4;
@@ -412,7 +419,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
   const ValueConsts vk = {held(0x64006400u), as_h2(held(0x2c002c00u)), as_h2(held(0xd400d400u))};
   // per row: maximum, sum, score that moves the maximum, exponent's offset
   float o[D / 16][NT][4];
-  float m[NT][2], l[NT][2], lim[NT][2], off[NT][2];
+  float m[NT][2], l[NT][2], lim[NT][2], off[NT][2], olo[X::FOLD ? NT : 1][2];
   auto clear = [&]() {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -423,6 +430,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
       m[nt][0] = m[nt][1] = -INFINITY;
       l[nt][0] = l[nt][1] = off[nt][0] = off[nt][1] = 0.0f;
       lim[nt][0] = lim[nt][1] = -INFINITY;
+      if constexpr (X::FOLD) olo[nt][0] = olo[nt][1] = 0.0f;
     }
   };
   clear();
@@ -616,8 +624,22 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
       }
 
       // ---- softmax: columns 2c, 2c + 1 are this lane's rows of queries -------
-      // m is the maximum of the scores as they are; a tile moves it only when one
-      // is beyond it by more than the slack, which each lane checks for its own
+      // m is the maximum of the scores as they are (FOLD: in powers of two, and
+      // with the value's scale); a tile moves it only when one is beyond it by
+      // more than the slack, which each lane checks for its own
+      float vs[U][2], vlo[U][2], vls[U][2];  // FOLD: s, lo and log2(s) of tokens r, r + 8
+      if constexpr (X::FOLD) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 f = __half22float2(
+                as_h2(reinterpret_cast<const uint32_t*>(st + u * MB + X::VP)[r + 8 * h]));
+            vs[u][h] = f.x;
+            vlo[u][h] = f.y;
+            vls[u][h] = lg2_approx(fmaxf(f.x, 5.9604644775390625e-8f));
+          }
+      }
       bool moved = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -629,31 +651,39 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
             for (int e = 0; e < 4; ++e)
               if (tok0 + 16 * u + r + 8 * (e >> 1) > last[e & 1]) z[u][nt][e] = -INFINITY;
         }
+      }
+      // what the maximum is taken of
+      auto rank = [&](int u, int nt, int e) {
+        return X::FOLD ? fmaf(z[u][nt][e], cmul[nt][e & 1], vls[u][e >> 1]) : z[u][nt][e];
+      };
+      float top[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          float v = fmaxf(z[0][nt][p], z[0][nt][2 + p]);
+          float v = fmaxf(rank(0, nt, p), rank(0, nt, 2 + p));
 #pragma unroll
-          for (int u = 1; u < U; ++u) v = fmaxf(v, fmaxf(z[u][nt][p], z[u][nt][2 + p]));
+          for (int u = 1; u < U; ++u) v = fmaxf(v, fmaxf(rank(u, nt, p), rank(u, nt, 2 + p)));
+          top[nt][p] = v;
           moved |= v > lim[nt][p];
         }
-      }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float f[2];
 #pragma unroll
           for (int p = 0; p < 2; ++p) {
-            float v = m[nt][p];
-#pragma unroll
-            for (int u = 0; u < U; ++u) v = fmaxf(v, fmaxf(z[u][nt][p], z[u][nt][2 + p]));
+            const float unit = X::FOLD ? 1.0f : cmul[nt][p];
+            float v = fmaxf(m[nt][p], top[nt][p]);
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
             // from -inf: nothing was summed yet (0 * 0 whatever the new one is)
-            f[p] = m[nt][p] == -INFINITY ? 0.0f : ex2_approx((m[nt][p] - v) * cmul[nt][p]);
+            f[p] = m[nt][p] == -INFINITY ? 0.0f : ex2_approx((m[nt][p] - v) * unit);
             l[nt][p] *= f[p];
+            if constexpr (X::FOLD) olo[nt][p] *= f[p];
             m[nt][p] = v;
-            lim[nt][p] = v + kPSlack / cmul[nt][p];
-            off[nt][p] = v == -INFINITY ? 0.0f : kPScale - v * cmul[nt][p];
+            lim[nt][p] = v + kPSlack / unit;
+            off[nt][p] = v == -INFINITY ? 0.0f : kPScale - v * unit;
           }
 #pragma unroll
           for (int i = 0; i < D / 16; ++i)
@@ -671,6 +701,10 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
           for (int e = 0; e < 4; ++e) {
             p[e] = ex2_approx(fmaf(z[u][nt][e], cmul[nt][e & 1], off[nt][e & 1]));
             l[nt][e & 1] += p[e];
+            if constexpr (X::FOLD) {
+              olo[nt][e & 1] = fmaf(p[e], vlo[u][e >> 1], olo[nt][e & 1]);
+              p[e] *= vs[u][e >> 1];
+            }
           }
           pf[u][nt][0] = transpose8x8(as_u32(__floats2half2_rn(p[0], p[1])));
           pf[u][nt][1] = transpose8x8(as_u32(__floats2half2_rn(p[2], p[3])));
@@ -685,7 +719,9 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
         for (int k = 0; k < 4; ++k) {
           const int tk = 2 * c + (k & 1) + 8 * (k >> 1);
           load_words<4 * VW>(v[k], mb + X::VR + tk * (D / 2) + r * (D / 16));
-          par[k] = reinterpret_cast<const uint32_t*>(mb + X::VP)[tk * NG + r * (D / 8) / GRP];
+          if constexpr (!X::FOLD)
+            par[k] = reinterpret_cast<const uint32_t*>(mb + X::VP)[tk * NG + r * (D / 8) / GRP];
+          else par[k] = 0;
         }
         const __half2 s0 = as_h2(__byte_perm(par[0], par[1], 0x5410));
         const __half2 o0 = as_h2(__byte_perm(par[0], par[1], 0x7632));
@@ -696,9 +732,18 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
 #pragma unroll
           for (int hi = 0; hi < 2; ++hi) {
             const uint32_t sel = hi ? 0x7632 : 0x5410;
+            const uint32_t b0 = __byte_perm(v[0][w], v[1][w], sel), b1 = __byte_perm(v[2][w], v[3][w], sel);
             uint32_t x0[4], x1[4];
-            value_pairs(__byte_perm(v[0][w], v[1][w], sel), s0, o0, vk, x0);
-            value_pairs(__byte_perm(v[2][w], v[3][w], sel), s1, o1, vk, x1);
+            if constexpr (X::FOLD) {
+              // n 2^-24, and 16 times that in the second rows
+              x0[0] = b0 & 0x000f000fu; x0[1] = b0 & 0x00f000f0u;
+              x1[0] = b1 & 0x000f000fu; x1[1] = b1 & 0x00f000f0u;
+              x0[2] = (b0 >> 8) & 0x000f000fu; x0[3] = (b0 >> 8) & 0x00f000f0u;
+              x1[2] = (b1 >> 8) & 0x000f000fu; x1[3] = (b1 >> 8) & 0x00f000f0u;
+            } else {
+              value_pairs(b0, s0, o0, vk, x0);
+              value_pairs(b1, s1, o1, vk, x1);
+            }
 #pragma unroll
             for (int q = 0; q < 2; ++q)
 #pragma unroll
@@ -718,7 +763,17 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l[nt][p] += __shfl_xor_sync(0xffffffffu, l[nt][p], x);
         if (bad) l[nt][p] = __int_as_float(0x7fc00000);
-        m[nt][p] *= cmul[nt][p];  // in powers of two from here on
+        if constexpr (X::FOLD) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) olo[nt][p] += __shfl_xor_sync(0xffffffffu, olo[nt][p], x);
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            o[i][nt][p] = fmaf(o[i][nt][p], 16777216.0f, olo[nt][p]);
+            o[i][nt][2 + p] = fmaf(o[i][nt][2 + p], 1048576.0f, olo[nt][p]);
+          }
+        } else {
+          m[nt][p] *= cmul[nt][p];  // in powers of two from here on
+        }
       }
     const bool whole = t0 == 0 && t1 == use.n;
     const int64_t seg = (int64_t)use.entry * a.c.Hk + head;

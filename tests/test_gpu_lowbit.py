@@ -436,6 +436,83 @@ def test_attention_small_values():
             + 2.0 ** -25).all()
 
 
+@pytest.mark.parametrize("dim,group", [(64, 64), (128, 32), (128, 128), (256, 64)])
+def test_attention_values_of_many_magnitudes(dim, group):
+    # tokens whose values differ by 2^20 in size, constant groups (scale 0) and
+    # zeros among them: what each contributes keeps its precision
+    g = gen(dim + group + 1)
+    n = 230
+    cache = b200k.KVCache4.zeros(16, 16, 2, dim, group)
+    k = randn(g, 256, 2, dim).half()
+    v = randn(g, 256, 2, dim) * torch.exp2(torch.randint(-12, 9, (256, 1, 1), generator=g, device="cuda"))
+    v[::5] = v[::5, :, :1]           # constant rows
+    v[::7] = 0
+    v = v.half()
+    b200k.kv_cache_write(cache, k, v, torch.arange(256, device="cuda"))
+    table = torch.arange(16, dtype=torch.int32, device="cuda")[None]
+    q = randn(g, 1, 1, 8, dim).half()
+    kv = values64(cache, k, v)
+    ro, _ = attend64(q, kv, table, [n], 16)
+    o = b200k.cache_attention(q, cache, table, torch.tensor([n], dtype=torch.int32, device="cuda"))
+    # each token's share is off by 2^-9 of itself
+    z = torch.einsum("hd,jhd->hj", q[0, 0].double(), kv[0][:n].repeat_interleave(4, 1)) * dim ** -0.5
+    share = torch.einsum("hj,jhd->hd", torch.softmax(z, -1), kv[1][:n].abs().amax(-1, keepdim=True)
+                         .expand(-1, -1, dim).repeat_interleave(4, 1))
+    assert ((o[0, 0].double() - ro[0, 0]).abs() <= 2.0 ** -9 * share + 2.0 ** -11 * ro[0, 0].abs()
+            + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("group", [32, 128])
+def test_attention_only_constant_values(group):
+    g = gen(21)
+    cache = b200k.KVCache4.zeros(8, 16, 1, 128, group)
+    k = randn(g, 128, 1, 128).half()
+    v = torch.full((128, 1, 128), 1.5, device="cuda").half()
+    b200k.kv_cache_write(cache, k, v, torch.arange(128, device="cuda"))
+    table = torch.arange(8, dtype=torch.int32, device="cuda")[None]
+    o, lse = b200k.cache_attention(randn(g, 1, 1, 4, 128).half(), cache, table,
+                                   torch.tensor([100], dtype=torch.int32, device="cuda"), return_lse=True)
+    assert (o.float() - 1.5).abs().max() <= 2.0 ** -10 and lse.isfinite().all()
+
+
+def test_attention_a_nan_token_is_not_seen_before_its_time():
+    # several queries: a token of NaN, written last, must not reach the rows
+    # before it (0 * NaN), nor what lies past the length any row
+    g = gen(22)
+    for dim, group in ((64, 32), (64, 64), (128, 32), (128, 128), (256, 128)):
+        cache, k, v = fill(g, 3, 2, 32, dim, group, torch.float16)
+        bad = torch.full((1, 2, dim), float("nan"), device="cuda", dtype=torch.float16)
+        b200k.kv_cache_write(cache, bad, bad, torch.tensor([69], device="cuda"))
+        table = torch.arange(3, dtype=torch.int32, device="cuda")[None]
+        q = randn(g, 1, 4, 8, dim).half()
+        o = b200k.cache_attention(q, cache, table, torch.tensor([71], dtype=torch.int32, device="cuda"))
+        # rows see up to 67, 68, 69, 70
+        assert o[0, :2].isfinite().all() and o[0, 2:].isnan().all()
+        # a value of NaN alone (its key is a number)
+        b200k.kv_cache_write(cache, k[69:70], bad, torch.tensor([69], device="cuda"))
+        o = b200k.cache_attention(q, cache, table, torch.tensor([71], dtype=torch.int32, device="cuda"))
+        assert o[0, :2].isfinite().all() and o[0, 2:].isnan().all()
+
+
+def test_attention_under_a_graph():
+    g = gen(23)
+    cache, k, v = fill(g, 40, 2, 32, 128, 64, torch.bfloat16)
+    table, lengths = make_tables(g, [900, 40], 32, 40)
+    q = randn(g, 2, 1, 8, 128).bfloat16()
+    want = b200k.cache_attention(q, cache, table, lengths)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = b200k.cache_attention(q, cache, table, lengths)
+    for n in ([900, 40], [17, 0], [1, 33]):
+        lengths.copy_(torch.tensor(n, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, b200k.cache_attention(q, cache, table, lengths))
+    lengths.copy_(torch.tensor([900, 40], dtype=torch.int32))
+    graph.replay()
+    assert torch.equal(got, want)
+
+
 def test_attention_strided_queries_and_another_stream():
     g = gen(16)
     cache, k, v = fill(g, 12, 2, 16, 128, 32, torch.float16)
