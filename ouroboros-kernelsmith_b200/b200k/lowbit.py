@@ -44,6 +44,16 @@ def _call(dev, fn, name, *args):
     L.check(st, name)
 
 
+def _new(m, n, dtype, dev):
+    """A fresh contiguous [m, n] (empty_strided takes the least time on the host)."""
+    return torch.empty_strided((m, n), (n, 1), dtype=dtype, device=dev)
+
+
+def _matrix(t, n):
+    """_rows, which a contiguous matrix need not pay for."""
+    return (t, n) if t.dim() == 2 and t.is_contiguous() and t.shape[1] == n else _rows(t, n)
+
+
 def _dt16(t: torch.dtype, what: str) -> int:
     try:
         return _DT16[t]
@@ -64,19 +74,19 @@ def _norm_quant(x, residual, w, dtype, group, eps):
     if group not in (None, 32, 64, 128):
         raise ValueError(f"b200k: group must be None, 32, 64 or 128, got {group}")
     n = x.shape[-1]
-    x2, ldx = _rows(x, n)
+    x2, ldx = _matrix(x, n)
     m = x2.shape[0]
     if residual is not None:
         if residual.shape != x.shape:
             raise ValueError(f"b200k: residual shape {tuple(residual.shape)} != {tuple(x.shape)}")
-        r2, ldr = _rows(residual, n)
-        h = torch.empty((m, n), dtype=x.dtype, device=dev)
+        r2, ldr = _matrix(residual, n)
+        h = _new(m, n, x.dtype, dev)
     else:
         r2, ldr, h = None, 0, None
     w1 = _vec(w, n, "weight")
     ns = 1 if group is None else (n + group - 1) // group
-    q = torch.empty((m, n), dtype=dtype, device=dev)
-    scale = torch.empty((m, ns), dtype=torch.float32, device=dev)
+    q = _new(m, n, dtype, dev)
+    scale = _new(m, ns, torch.float32, dev)
     _call(dev, L.lib.b2k_norm_quant, "b2k_norm_quant", _p(x2), ldx, _p(r2), ldr, _p(w1), _p(h), n,
           _p(q), n, _p(scale), ns, m, n, dt, qt, group or 0, eps)
     if x.dim() != 2:
@@ -180,7 +190,7 @@ def kv_cache_write(cache: KVCache4, k, v, slots) -> None:
     dt = _dt16(k.dtype, "k and v")
     hk, d = cache.kv_heads, cache.head_dim
     for t in (k, v):
-        if t.dim() < 2 or t.shape[-2:] != (hk, d):
+        if t.shape[-2:] != (hk, d):
             raise ValueError(f"b200k: k and v must be [..., {hk}, {d}], got {tuple(t.shape)}")
     if k.shape != v.shape:
         raise ValueError(f"b200k: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
@@ -205,9 +215,8 @@ def kv_cache_read(cache: KVCache4, slots, *, dtype: torch.dtype = torch.bfloat16
     dev = _cuda(cache.data, slots)
     dt = _dt16(dtype, "dtype")
     s1 = _check_slots(slots, None)
-    shape = tuple(slots.shape) + (cache.kv_heads, cache.head_dim)
-    k = torch.empty(shape, dtype=dtype, device=dev)
-    v = torch.empty(shape, dtype=dtype, device=dev)
+    k = torch.empty((*slots.shape, cache.kv_heads, cache.head_dim), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
     _call(dev, L.lib.b2k_kv4_read, "b2k_kv4_read", *cache._args, s1.data_ptr(), s1.shape[0],
           k.data_ptr(), v.data_ptr(), dt)
     return k, v
@@ -242,14 +251,14 @@ def cache_attention(q, cache: KVCache4, page_table, lengths, *, scale: float | N
     if q.stride(3) != 1:
         q = q.contiguous()
     page_table, lengths = page_table.contiguous(), lengths.contiguous()
-    o = torch.empty((b, sq, h, d), dtype=q.dtype, device=dev)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((b, h, sq), dtype=torch.float32, device=dev) if return_lse else None
     nws = cache._sizes.get((b, sq, h))
     if nws is None:
         with _dev(dev):
             nws = L.lib.b2k_kv4_attention_workspace(b, sq, h, hk, d)
         cache._sizes[(b, sq, h)] = nws
-    ws = torch.empty((nws,), dtype=torch.uint8, device=dev) if nws > 0 else None
+    ws = _new(1, nws, torch.uint8, dev) if nws > 0 else None
     _call(dev, L.lib.b2k_kv4_attention, "b2k_kv4_attention", q.data_ptr(), *q.stride()[:3], o.data_ptr(),
           _p(lse), *cache._args, page_table.data_ptr(), page_table.shape[1], lengths.data_ptr(), b, sq, h,
           d ** -0.5 if scale is None else scale, 1 if causal else 0, dt, _p(ws), nws)
@@ -368,7 +377,7 @@ def w4_matmul(x, weight: W4Weight, *, x_scale=None, out_dtype: torch.dtype | Non
     if x.dim() < 1 or x.shape[-1] != k:
         raise ValueError(f"b200k: x {tuple(x.shape)} does not end in {k} columns")
     if x.numel():
-        x2, ldx = _rows(x, k)
+        x2, ldx = _matrix(x, k)
         m = x2.shape[0]
     else:  # no rows, or no columns
         x2, ldx, m = x, k, math.prod(x.shape[:-1])
@@ -398,13 +407,13 @@ def w4_matmul(x, weight: W4Weight, *, x_scale=None, out_dtype: torch.dtype | Non
         out_dtype = x.dtype if out_dtype is None else out_dtype
     if out_dtype not in _DT:
         raise TypeError(f"b200k: unsupported out_dtype {out_dtype}")
-    y = torch.empty((m, n), dtype=out_dtype, device=dev)
+    y = _new(m, n, out_dtype, dev)
     nws = weight._sizes.get((m, xt))
     if nws is None:
         with _dev(dev):
             nws = L.lib.b2k_w4_matmul_workspace(m, n, k, group, xt)
         weight._sizes[(m, xt)] = nws
-    ws = torch.empty((nws,), dtype=torch.uint8, device=dev) if nws > 0 else None
+    ws = _new(1, nws, torch.uint8, dev) if nws > 0 else None
     _call(dev, L.lib.b2k_w4_matmul, "b2k_w4_matmul", x2.data_ptr(), ldx, xt, _p(xs), ldxs, xg,
           *weight._args, m, n, k, y.data_ptr(), n, _DT[out_dtype], _p(ws), nws)
     return y if x.dim() == 2 else y.view(x.shape[:-1] + (n,))

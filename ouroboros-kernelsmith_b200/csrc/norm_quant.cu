@@ -379,7 +379,7 @@ template <typename T, bool I8, bool RESID, bool GROUPED>
 static bool norm_quant_try_pipe(const NormQuantArgs& a, cudaStream_t st) {
   constexpr int E = Traits<T>::E, NIN = RESID ? 2 : 1;
   const int64_t nvec = a.N / E, row_bytes = a.N * (int64_t)sizeof(T);
-  if (!a.aligned || (RESID && !a.h) || nvec < 256) return false;
+  if (!a.aligned || (RESID && !a.h) || nvec < 256 || a.M < sm_count()) return false;
   // Two vectors per thread up to 256 threads, then four (16381 x 8192 bf16:
   // 199 us with two, 148 with four; 8192 x 4096 fp16 with its reading back: 61
   // and 62).  Compiled for 768 threads a kernel has at most 80 registers: more
@@ -407,7 +407,8 @@ template <typename T, bool I8> static int norm_quant_launch(const NormQuantArgs&
                                     : norm_quant_try_pipe<T, I8, false, false>(a, st));
   if (piped) return check_launch("b2k_norm_quant");
   RowCfg cfg;
-  if (!choose_row_cfg(a.N, E, 128, &cfg, 4, 512)) {
+  // few rows: as many threads as a row has vectors, for the latency
+  if (!choose_row_cfg(a.N, E, a.M < sm_count() ? 512 : 128, &cfg, 4, 512)) {
     launch_pdl(norm_quant_stream_kernel<T, I8>, dim3((unsigned)a.M), dim3(1024), 0, st, a);
     return check_launch("b2k_norm_quant");
   }
