@@ -2,20 +2,24 @@
 // paged cache (kv4.cuh), any set of slots in any order.
 //
 // One thread holds 8 dimensions of a row (16 bytes on one side, one 32-bit
-// word of nibbles on the other); g / 8 neighbouring lanes reduce their group's
-// minimum and maximum with shuffles.  A block takes 16 tokens, keys and
-// values, and every thread kKvHeads heads, so it has that many loads in flight
-// and a prefill's writes fill whole micro blocks.  Both are bound by HBM: 2 D
-// Hk values of T on one side, Hk (D + 8 D / g) bytes on the other; close to
-// that the instructions per element count too, hence the packed 16-bit
-// arithmetic below.
+// word of nibbles on the other) of several heads in turn; g / 8 neighbouring
+// lanes reduce their group's minimum and maximum with shuffles.  A block takes
+// a few tokens, keys and values.  Both are bound by HBM: 2 D Hk values of T on
+// one side, Hk (D + 8 D / g) bytes on the other.  Close to that the
+// instructions per element count too, hence the packed 16-bit and fp32
+// arithmetic below: 30011 tokens of 8 heads of 128 (fp16, g 32) take 76 us to
+// write and to read back (30 us of it the reading), whose bytes take 49 us at
+// the copy bandwidth; the write issues in 77 % of its cycles.
 #include "kv4.cuh"
 #include "rowio.cuh"
 #include "tma.cuh"
 
 namespace b2k {
 
-constexpr int kKvHeads = 4;
+// Heads of a thread.  A read has all of its in flight at once; a write takes
+// kAhead at a time, as its arithmetic wants the registers.
+constexpr int kReadHeads = 4, kAhead = 2;
+constexpr int kTokens = 4;  // of a block (30011 tokens written and read back: 76 us, 78 with 8)
 
 struct Kv4IoArgs {
   Kv4 c;
@@ -26,6 +30,7 @@ struct Kv4IoArgs {
   int64_t T;
   int64_t ldk, hdk, ldv, hdv;  // token and head strides in elements
   int aligned;
+  int heads;  // of a block
 };
 
 // this thread's row: its token, keys or values, and where the token's slot
@@ -36,13 +41,13 @@ struct Kv4Row {
   bool live, in, padding;
   unsigned char *bits, *par;  // of head 0: the row's words, its parameters
 };
-template <int D> __device__ __forceinline__ Kv4Row kv4_row(const Kv4IoArgs& a) {
+template <int D> __device__ __forceinline__ Kv4Row kv4_row(const Kv4IoArgs& a, int heads) {
   constexpr int W = D / 8;
   Kv4Row p;
   p.word = threadIdx.x % W;
-  p.token = (int64_t)blockIdx.x * 16 + threadIdx.x / W;
+  p.token = (int64_t)blockIdx.x * kTokens + threadIdx.x / W;
   p.is_v = threadIdx.y;
-  p.head = blockIdx.y * kKvHeads;
+  p.head = blockIdx.y * heads;
   p.live = p.token < a.T;
   const int64_t slot = p.live ? a.slots[p.token] : -1;
   p.padding = slot < 0;
@@ -77,33 +82,39 @@ template <> struct Pair16<__nv_bfloat16> {
 // n = clamp(rint(d / s), 0, 15) of eight values, as nibbles, for s > 0 a
 // float16.  The product with 1 / s and its rounding give n exactly except
 // where the quotient is (almost) halfway between two integers (the product is
-// off by 2^-22 of itself, 3e-6 at most).  d - n s, whose terms fit fp32 (n s
-// has 15 bits), tells whether any of the eight is that near; then its
-// comparison with s / 2 decides, ties to even.
-__device__ __forceinline__ uint32_t kv4_round8(const float* x, float lo, float s) {
-  constexpr float kShift = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer
-  const float r = rcp_approx(s) * (1.0f / 15.0f), half = 0.5f * s, safe = half * (1.0f - 1e-5f);
-  uint32_t bits = 0;
+// off by 2^-22 of itself, 3e-6 at most) or outside the range (where lo was
+// rounded by more than s / 2).  d - n s, whose terms fit fp32 (n s has 15
+// bits), tells whether any of the eight is that near; then its comparison with
+// s / 2 decides, ties to even.
+__device__ __forceinline__ uint32_t kv4_round8(const float2* x, float lo, float s) {
+  constexpr float kShift = 12582912.0f;      // 1.5 * 2^23: adding it rounds to an integer
+  constexpr uint32_t kBits = 0x4b400000u;    // its bits; the integer lies in the low ones
+  const float r = rcp_approx(s), half = 0.5f * s, safe = half * (1.0f - 1e-5f);
+  uint32_t bits = 0, all = 0;
   bool near = false;
 #pragma unroll
-  for (int e = 7; e >= 0; --e) {
-    const float d = x[e] - lo;
-    const float t = fmaf(__saturatef(d * r), 15.0f, kShift);
-    near |= fabsf(fmaf(kShift - t, s, d)) >= safe;
-    bits = bits * 16u + __float_as_uint(t);  // 0x4b400000 + n
+  for (int e = 3; e >= 0; --e) {
+    const float2 d = add2(x[e], f2s(-lo));
+    const float2 t = fma2(d, f2s(r), f2s(kShift));
+    const float2 rest = fma2(sub2(f2s(kShift), t), f2s(s), d);
+    near |= fabsf(rest.x) >= safe;
+    near |= fabsf(rest.y) >= safe;
+    const uint32_t a = __float_as_uint(t.x), b = __float_as_uint(t.y);
+    bits = bits * 256u + b * 16u + a;
+    all |= (a ^ kBits) | (b ^ kBits);
   }
-  bits -= 0x4b400000u * 0x11111111u;
-  if (near) {
-    uint32_t fixed = 0;
+  bits -= kBits * 0x11111111u;
+  if (near || all > 15u) {
+    bits = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      uint32_t q = (bits >> (4 * e)) & 15u;
-      const float rest = fmaf(-(float)q, s, x[e] - lo);
+      const float d = (e & 1 ? x[e >> 1].y : x[e >> 1].x) - lo;
+      const float n = fminf(fmaxf(rintf(d * r), 0.0f), 15.0f), rest = fmaf(-n, s, d);
+      uint32_t q = (uint32_t)n;
       if (fabsf(rest) > half || (fabsf(rest) == half && (q & 1u)))
         q = rest > 0.0f ? min(q + 1u, 15u) : q - (q > 0u ? 1u : 0u);
-      fixed |= q << (4 * e);
+      bits |= q << (4 * e);
     }
-    bits = fixed;
   }
   return bits;
 }
@@ -120,35 +131,31 @@ __device__ __forceinline__ __half kv4_step(float d) {
 }
 
 template <typename T, int D, int LANES>
-__global__ void __launch_bounds__(4 * D, 1536 / (4 * D)) kv4_write_kernel(const __grid_constant__ Kv4IoArgs a) {
+__global__ void __launch_bounds__(kTokens * D / 4, 5 * 1024 / (kTokens * D)) kv4_write_kernel(const __grid_constant__ Kv4IoArgs a) {
   using P = Pair16<T>;
   griddep_launch_dependents();
   griddep_wait();
-  const Kv4Row p = kv4_row<D>(a);
-  const T* src = p.is_v ? static_cast<const T*>(a.v) + p.token * a.ldv + p.head * a.hdv
-                        : static_cast<const T*>(a.k) + p.token * a.ldk + p.head * a.hdk;
+  Kv4Row p = kv4_row<D>(a, a.heads);
+  const int heads = min(a.heads, a.c.Hk - p.head);  // of this block
   const int64_t hd = p.is_v ? a.hdv : a.hdk;
-  uint4 raw[kKvHeads];
-#pragma unroll
-  for (int h = 0; h < kKvHeads; ++h) {
-    raw[h] = zero4();
-    if (p.live && p.head + h < a.c.Hk) {
-      const T* from = src + h * hd + p.word * 8;
-      if (a.aligned) {
-        raw[h] = ld_stream(from);
-      } else {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = ld1(from + e);
-        raw[h] = pack<T>(x);
-      }
-    }
-  }
+  const T* src = (p.is_v ? static_cast<const T*>(a.v) + p.token * a.ldv
+                         : static_cast<const T*>(a.k) + p.token * a.ldk) + p.head * hd + p.word * 8;
   const int64_t head_bytes = (int64_t)(a.c.P >> 4) * a.c.micro_bytes();
+  auto load = [&](int h) {
+    if (!p.live || h >= heads) return zero4();
+    const T* from = src + h * hd;
+    if (a.aligned) return ld_stream(from);
+    float x[8];
 #pragma unroll
-  for (int h = 0; h < kKvHeads; ++h) {
+    for (int e = 0; e < 8; ++e) x[e] = ld1(from + e);
+    return pack<T>(x);
+  };
+  uint4 raw[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) raw[i] = load(i);
+  auto one = [&](const uint4& row) {
     // minimum and minus maximum of the group, as a pair
-    const typename P::type* w = reinterpret_cast<const typename P::type*>(&raw[h]);
+    const typename P::type* w = reinterpret_cast<const typename P::type*>(&row);
     const typename P::type mn = __hmin2_nan(__hmin2_nan(w[0], w[1]), __hmin2_nan(w[2], w[3]));
     const typename P::type mx = __hmax2_nan(__hmax2_nan(w[0], w[1]), __hmax2_nan(w[2], w[3]));
     typename P::type ends = P::pair(__hmin_nan(P::low(mn), P::high(mn)),
@@ -159,45 +166,59 @@ __global__ void __launch_bounds__(4 * D, 1536 / (4 * D)) kv4_write_kernel(const 
       ends = __hmin2_nan(ends, *reinterpret_cast<typename P::type*>(&t));
     }
     const float2 f = P::f(ends);
-    float lo = f.x, hi = -f.y, x[8];
-    unpack<T>(raw[h], x);
+    float lo = f.x, hi = -f.y;
+    float2 x[4];
+    unpack2<T>(row, x);
     if (!(lo >= -kKv4Limit && hi <= kKv4Limit)) {  // beyond the range, or a NaN
       lo = min_nan(max_nan(lo, -kKv4Limit), kKv4Limit);
       hi = min_nan(max_nan(hi, -kKv4Limit), kKv4Limit);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = min_nan(max_nan(x[e], -kKv4Limit), kKv4Limit);
+      for (int e = 0; e < 4; ++e) {
+        x[e].x = min_nan(max_nan(x[e].x, -kKv4Limit), kKv4Limit);
+        x[e].y = min_nan(max_nan(x[e].y, -kKv4Limit), kKv4Limit);
+      }
     }
     const __half sh = kv4_step(hi - lo), lh = __float2half_rn(lo);
     const float s = __half2float(sh);
     // a constant group has n = 0, and so has a NaN one
     const uint32_t bits = s > 0.0f ? kv4_round8(x, __half2float(lh), s) : 0u;
     // a slot outside the pool (negative: padding) is not written
-    if (!p.in || p.head + h >= a.c.Hk) continue;
-    *reinterpret_cast<uint32_t*>(p.bits + h * head_bytes) = bits;
-    if ((p.word & (LANES - 1)) == 0)
-      *reinterpret_cast<__half2*>(p.par + h * head_bytes) = __halves2half2(sh, lh);
-  }
+    if (p.in) {
+      *reinterpret_cast<uint32_t*>(p.bits) = bits;
+      if ((p.word & (LANES - 1)) == 0) *reinterpret_cast<__half2*>(p.par) = __halves2half2(sh, lh);
+    }
+    p.bits += head_bytes;
+    p.par += head_bytes;
+  };
+  for (int h = 0; h < heads; h += kAhead)
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (h + i < heads) {
+        const uint4 row = raw[i];
+        raw[i] = load(h + i + kAhead);
+        one(row);
+      }
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(4 * D) kv4_read_kernel(const __grid_constant__ Kv4IoArgs a) {
+__global__ void __launch_bounds__(kTokens * D / 4) kv4_read_kernel(const __grid_constant__ Kv4IoArgs a) {
   static_assert(Traits<T>::E == 8, "16-bit outputs");
   griddep_launch_dependents();
   griddep_wait();
-  const Kv4Row p = kv4_row<D>(a);
+  const Kv4Row p = kv4_row<D>(a, kReadHeads);
   if (!p.live) return;
   const int64_t head_bytes = (int64_t)(a.c.P >> 4) * a.c.micro_bytes();
-  uint32_t bits[kKvHeads];
-  __half2 par[kKvHeads];
+  uint32_t bits[kReadHeads];
+  __half2 par[kReadHeads];
 #pragma unroll
-  for (int h = 0; h < kKvHeads; ++h)
+  for (int h = 0; h < kReadHeads; ++h)
     if (p.in && p.head + h < a.c.Hk) {
       bits[h] = __ldcs(reinterpret_cast<const uint32_t*>(p.bits + h * head_bytes));
       par[h] = __ldcs(reinterpret_cast<const __half2*>(p.par + h * head_bytes));
     }
   T* dst = static_cast<T*>(p.is_v ? a.vo : a.ko) + (p.token * a.c.Hk + p.head) * D + p.word * 8;
 #pragma unroll
-  for (int h = 0; h < kKvHeads; ++h) {
+  for (int h = 0; h < kReadHeads; ++h) {
     if (p.head + h >= a.c.Hk) continue;
     uint4 out;
     uint32_t* w = &out.x;
@@ -267,8 +288,18 @@ int kv4_check(const char* what, const void* data, int64_t pages, int64_t Hk, int
   return B2K_OK;
 }
 
-template <typename T, int D> static void kv4_launch_d(const Kv4IoArgs& a, bool write, cudaStream_t st) {
-  const dim3 grid((unsigned)((a.T + 15) / 16), (a.c.Hk + kKvHeads - 1) / kKvHeads), block(2 * D, 2);
+template <typename T, int D> static void kv4_launch_d(Kv4IoArgs a, bool write, cudaStream_t st) {
+  const int64_t chunks = (a.T + kTokens - 1) / kTokens;
+  a.heads = kReadHeads;
+  if (write) {
+    // a thread's own costs (its slot, its place) are those of several heads: as
+    // many of them as leave six blocks per SM (30011 tokens written and read
+    // back: 89 us with two heads a thread, 78 with all eight; 64 tokens take
+    // two)
+    for (a.heads = a.c.Hk; a.heads > 2 && chunks * ((a.c.Hk + a.heads - 1) / a.heads) < 6 * sm_count();)
+      a.heads = (a.heads + 1) / 2;
+  }
+  const dim3 grid((unsigned)chunks, (a.c.Hk + a.heads - 1) / a.heads), block(kTokens * D / 8, 2);
   if (!write) launch_pdl(kv4_read_kernel<T, D>, grid, block, 0, st, a);
   else if (a.c.g == 32) launch_pdl(kv4_write_kernel<T, D, 4>, grid, block, 0, st, a);
   else if (a.c.g == 64) launch_pdl(kv4_write_kernel<T, D, 8>, grid, block, 0, st, a);

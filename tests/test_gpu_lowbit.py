@@ -831,3 +831,30 @@ def test_refusals():
         b200k.w4_pack(torch.zeros(4, 64, dtype=torch.uint8, device="cuda"), torch.ones(4, 3, **f16), group=32)
     with pytest.raises(ValueError):
         b200k.W4Weight(wt.tiles, wt.scales, wt.zeros, 33, 64)
+
+
+# --------------------------------------------------------------------------
+# the rounding of the cache, where it is hardest
+@pytest.mark.parametrize("dtype", T16)
+@pytest.mark.parametrize("group", [32, 64])
+def test_cache_rounding_at_ties_offsets_and_small_ranges(dtype, group):
+    g = gen(31)
+    rows = []
+    for s in (1.0, 0.25, 2.0 ** -9, 8.0):             # exact ties: multiples of s / 2
+        rows.append(torch.randint(0, 31, (64, 64), generator=g, device="cuda") * (s / 2))
+    rows.append(1000 + 0.01 * randn(g, 64, 64))       # the minimum's rounding exceeds the step
+    rows.append(-3000 + 4 * randn(g, 64, 64))
+    rows.append(1e-5 * randn(g, 64, 64))              # subnormal steps
+    rows.append(6e4 * randn(g, 64, 64).clamp(-1, 1))
+    x = torch.cat(rows).to(dtype)[:, None].contiguous()     # [tokens, 1, 64]
+    n = x.shape[0]
+    cache = b200k.KVCache4.zeros(-(-n // 16), 16, 1, 64, group)
+    slots = torch.arange(n, device="cuda")
+    b200k.kv_cache_write(cache, x, x, slots)
+    for got in values64(cache, x, x):
+        t, s, lo = quantise64(x, group)
+        want = lo + t.round() * s                     # ties to even, as stored
+        got = got[:n].unflatten(-1, (-1, group))
+        off = (got - want).abs() > s * 2.0 ** -20
+        near = ((t - t.floor() - 0.5).abs() < 2.0 ** -22) & ((t - t.floor() - 0.5) != 0)
+        assert not (off & ~near).any()
