@@ -33,7 +33,8 @@
 //     range whatever the values' magnitude.  (8 x 65536 tokens, D 128, g 128: 118
 //     us instead of 135.)
 //     For float16 queries the probabilities take two products, p rounded and
-//     what that left: their rounding would show beside float16's own.
+//     what that left: their rounding would show beside float16's own (32 x 8192
+//     tokens, g 32: 92 us instead of 84).
 //   * The running maximum and sum are fp32, per lane for its own tokens; the
 //     output is rescaled only when a row's maximum has moved by 2^4.
 //
