@@ -115,9 +115,24 @@ def add_rmsnorm_quant(x, residual, w, *, dtype: torch.dtype = torch.int8,
     return _norm_quant(x, residual, w, dtype, group, eps)
 
 
+class _Handle:
+    """What the kernels are called with is taken from the tensors once, when the
+    handle is made, so its attributes stay what they are."""
+
+    __slots__ = ()
+
+    def _fill(self, **values):
+        for name, value in values.items():
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"b200k: {type(self).__name__}.{name} cannot be set; make a new "
+                             f"{type(self).__name__}")
+
+
 # --------------------------------------------------------------------------
 # the 4-bit cache (b2k_kv4_write, b2k_kv4_read, b2k_kv4_attention)
-class KVCache4:
+class KVCache4(_Handle):
     """A paged key/value cache in 4 bits: `data`, uint8
     [pages, kv_heads, page_size / 16, 16 * (D + 8 * D / group)].
 
@@ -146,12 +161,11 @@ class KVCache4:
                 or not data.is_contiguous():
             raise ValueError("b200k: cache data must be contiguous [pages, kv_heads, "
                              f"page_size / 16, {micro}], got {tuple(data.shape)}")
-        self.data = data
-        self.pages, self.kv_heads = data.shape[0], data.shape[1]
-        self.page_size = 16 * data.shape[2]
-        self.head_dim, self.group = head_dim, group
-        self._args = (data.data_ptr(), self.pages, self.kv_heads, self.page_size, head_dim, group)
-        self._sizes = {}  # workspace bytes of cache_attention by (B, Sq, H)
+        pages, kv_heads, page_size = data.shape[0], data.shape[1], 16 * data.shape[2]
+        self._fill(data=data, pages=pages, kv_heads=kv_heads, page_size=page_size,
+                   head_dim=head_dim, group=group,
+                   _args=(data.data_ptr(), pages, kv_heads, page_size, head_dim, group),
+                   _sizes={})  # workspace bytes of cache_attention by (B, Sq, H)
 
     @classmethod
     def zeros(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, group: int = 32,
@@ -267,7 +281,7 @@ def cache_attention(q, cache: KVCache4, page_table, lengths, *, scale: float | N
 
 # --------------------------------------------------------------------------
 # 4-bit weights (b2k_w4_pack, b2k_w4_quantize, b2k_w4_matmul)
-class W4Weight:
+class W4Weight(_Handle):
     """Weights [n, k] in 4 bits, laid out for w4_matmul: w = scale * (i - zero)
     for integers i in 0..15, scale and zero (8 without zeros) per row and group
     of 32, 64 or 128 columns.
@@ -299,10 +313,10 @@ class W4Weight:
             if t is not None and (not t.is_contiguous() or t.data_ptr() % 16):
                 raise ValueError("b200k: tiles, scales and zeros must be contiguous and 16-byte "
                                  "aligned")
-        self.tiles, self.scales, self.zeros = tiles, scales, zeros
-        self.n, self.k, self.group = n, k, 128 // scales.shape[2]
-        self._args = (_p(tiles), _p(scales), _p(zeros), st, self.group)
-        self._sizes = {}  # workspace bytes of w4_matmul by (rows, x's type)
+        group = 128 // scales.shape[2]
+        self._fill(tiles=tiles, scales=scales, zeros=zeros, n=n, k=k, group=group,
+                   _args=(_p(tiles), _p(scales), _p(zeros), st, group),
+                   _sizes={})  # workspace bytes of w4_matmul by (rows, x's type)
 
 
 def _w4_empty(n, k, group, stype, with_zeros, dev):

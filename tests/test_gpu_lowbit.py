@@ -858,3 +858,14 @@ def test_cache_rounding_at_ties_offsets_and_small_ranges(dtype, group):
         off = (got - want).abs() > s * 2.0 ** -20
         near = ((t - t.floor() - 0.5).abs() < 2.0 ** -22) & ((t - t.floor() - 0.5) != 0)
         assert not (off & ~near).any()
+
+
+def test_handles_cannot_be_repointed():
+    cache = b200k.KVCache4.zeros(2, 16, 1, 64)
+    weight = b200k.w4_quantize(torch.ones((16, 32), device="cuda"), group=32)
+    for handle in (cache, weight):
+        for name in handle.__slots__:
+            with pytest.raises(AttributeError):
+                setattr(handle, name, None)
+        with pytest.raises(AttributeError):
+            handle.other = 1
