@@ -6,7 +6,7 @@
 //   a = max |y| over the row / group;  scale = a / Q;  q = round(y Q / a)
 //   (Q = 127 for int8, 448 for e4m3; a < 1e-30: scale 0 and q 0)
 //
-// y stays in fp32 between the norm and its quantisation (one rounding).
+// y is quantised from fp32, as h w times Q / max |h w|: rs drops out of q.
 // Multiplying by rs > 0 and rounding are monotone, so max |y| is exactly
 // rs * max |h w|: the sum of squares and the row's maximum come out of ONE
 // block reduction, and the row is read once.  Bound by HBM: 2 reads and one
@@ -41,20 +41,24 @@ __device__ __forceinline__ float max_mag(float m, float v) {
   return r;
 }
 
-// scale and multiplier of a row or group whose largest |y| is `a`
-template <bool I8> __device__ __forceinline__ void quant_scale(float a, float& scale, float& inv) {
+// Scale, and multiplier of h w, of a row or group whose largest |h w| is `m`:
+// q = round(y Q / a) is round(h w Q / m), without the norm's own rounding (h w
+// is exact for 16-bit h and w, which leaves two roundings before the last).
+template <bool I8>
+__device__ __forceinline__ void quant_scale(float m, float rs, float& scale, float& mul) {
   constexpr float Q = I8 ? 127.0f : 448.0f;
+  const float a = m * rs;
   if (a < kQuantTiny) {
     scale = 0.0f;
-    inv = 0.0f;
+    mul = 0.0f;
   } else {  // a NaN goes on into scale and values
     scale = __fdiv_rn(a, Q);
-    inv = __fdiv_rn(Q, a);
+    mul = a == a ? __fdiv_rn(Q, m) : a;
   }
 }
 
 // E values -> E bytes.  The saturating conversions round to nearest even;
-// |v| <= Q up to one rounding of v = y * inv.
+// |v| <= Q up to the roundings of v = h w Q / m.
 template <bool I8, int E> __device__ __forceinline__ void quant_pack(const float* v, uint32_t* out) {
 #pragma unroll
   for (int k = 0; k < E / 4; ++k) {
@@ -127,8 +131,8 @@ __device__ __forceinline__ void group_sum_max(float& ss, uint32_t& mx, const Gro
 // the row); every lane of the warp calls it.  `width` lanes share a group.
 template <bool I8, int E>
 __device__ __forceinline__ void quant_slot(const NormQuantArgs& a, int64_t row, int64_t c, float* v,
-                                           float rs, float row_inv, int width) {
-  float inv = row_inv;
+                                           float rs, float row_mul, int width) {
+  float mul = row_mul;
   if (a.group) {
     float mf = 0.0f;
 #pragma unroll
@@ -136,12 +140,11 @@ __device__ __forceinline__ void quant_slot(const NormQuantArgs& a, int64_t row, 
     uint32_t m = __float_as_uint(mf);
     for (int o = width >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     float scale;
-    quant_scale<I8>(__uint_as_float(m) * rs, scale, inv);
+    quant_scale<I8>(__uint_as_float(m), rs, scale, mul);
     if (c < a.N && c % a.group == 0) a.scale[row * a.lds + c / a.group] = scale;
   }
-  const float f = rs * inv;
 #pragma unroll
-  for (int e = 0; e < E; ++e) v[e] *= f;
+  for (int e = 0; e < E; ++e) v[e] *= mul;
   quant_store<I8, E>(static_cast<uint8_t*>(a.q) + row * a.ldq, c, a.N, a.aligned != 0, v);
 }
 
@@ -191,10 +194,10 @@ __global__ void __launch_bounds__(1024) norm_quant_rows_kernel(NormQuantArgs a) 
   uint32_t mx = __float_as_uint(top);
   group_sum_max(ss, mx, g, red);
   const float rs = rsqrtf(ss / (float)a.N + a.eps);
-  float inv = 0.0f;
+  float mul = 0.0f;
   if (!a.group) {
     float scale;
-    quant_scale<I8>(__uint_as_float(mx) * rs, scale, inv);
+    quant_scale<I8>(__uint_as_float(mx), rs, scale, mul);
     if (live && g.tx == 0) a.scale[row * a.lds] = scale;
   }
   const int lanes = a.group / E;
@@ -202,7 +205,7 @@ __global__ void __launch_bounds__(1024) norm_quant_rows_kernel(NormQuantArgs a) 
 #pragma unroll
   for (int k = 0; k < V; ++k) {
     const int64_t c = ((int64_t)k * g.G + g.tx) * E;
-    quant_slot<I8, E>(a, row, live ? c : a.N, v[k], rs, inv, width);
+    quant_slot<I8, E>(a, row, live ? c : a.N, v[k], rs, mul, width);
   }
 }
 
@@ -245,10 +248,10 @@ __global__ void __launch_bounds__(1024) norm_quant_stream_kernel(NormQuantArgs a
   uint32_t mx = __float_as_uint(top);
   group_sum_max(ss, mx, g, red);
   const float rs = rsqrtf(ss / (float)a.N + a.eps);
-  float inv = 0.0f;
+  float mul = 0.0f;
   if (!a.group) {
     float scale;
-    quant_scale<I8>(__uint_as_float(mx) * rs, scale, inv);
+    quant_scale<I8>(__uint_as_float(mx), rs, scale, mul);
     if (g.tx == 0) a.scale[row * a.lds] = scale;
   }
   // whole warps stay in the loop: a group's lanes reduce together
@@ -259,7 +262,7 @@ __global__ void __launch_bounds__(1024) norm_quant_stream_kernel(NormQuantArgs a
     load_vec<T, false>(w, wr, c, a.N, al);
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] *= w[e];
-    quant_slot<I8, E>(a, row, c, v, rs, inv, a.group / E);
+    quant_slot<I8, E>(a, row, c, v, rs, mul, a.group / E);
   }
 }
 
@@ -348,9 +351,9 @@ __global__ void __launch_bounds__(THREADS) norm_quant_pipe_kernel(const __grid_c
       if constexpr (!GROUPED) mx = max(mx, __float_as_uint(t.y));
     }
     const float rs = rsqrtf(ss / (float)N + a.eps);
-    float inv = 0.0f, scale;
+    float mul = 0.0f, scale;
     if constexpr (!GROUPED) {
-      quant_scale<I8>(__uint_as_float(mx) * rs, scale, inv);
+      quant_scale<I8>(__uint_as_float(mx), rs, scale, mul);
       if (tx == 0) a.scale[row * a.lds] = scale;
     }
     uint8_t* qrow = static_cast<uint8_t*>(a.q) + row * a.ldq;
@@ -363,10 +366,10 @@ __global__ void __launch_bounds__(THREADS) norm_quant_pipe_kernel(const __grid_c
         for (int j = 0; j < H; ++j) m = max_mag(max_mag(m, v[k][j].x), v[k][j].y);
         uint32_t mb = __float_as_uint(m);
         for (int o = width >> 1; o > 0; o >>= 1) mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, o));
-        quant_scale<I8>(__uint_as_float(mb) * rs, scale, inv);
+        quant_scale<I8>(__uint_as_float(mb), rs, scale, mul);
         if (c < N && (c & (a.group - 1)) == 0) a.scale[row * a.lds + (c >> gshift)] = scale;
       }
-      const float2 f = f2s(rs * inv);
+      const float2 f = f2s(mul);
 #pragma unroll
       for (int j = 0; j < H; ++j) v[k][j] = mul2(v[k][j], f);
       quant_store<I8, E>(qrow, c, N, true, reinterpret_cast<const float*>(v[k]));
