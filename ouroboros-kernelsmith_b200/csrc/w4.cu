@@ -674,10 +674,13 @@ template <typename T> __global__ void __launch_bounds__(256) w4_sum_kernel(const
 }
 
 // How a product is split.  One block per SM, its warps' rings as deep as shared
-// memory allows beside x (2 to kW4Stages stages); K is split over blocks where x does not fit beside that.  x is
-// prepared once by a kernel of its own where every block's own preparation
-// would take it more than kW4Own eights of columns per thread.
-constexpr int kW4Own = 4;
+// memory allows beside x (2 to kW4Stages stages); K is split over blocks where
+// x does not fit beside that.  x is prepared once by a kernel of its own where
+// every block's own preparation would take it more than kW4Own eights of
+// columns per thread (own preparation against the kernel: 1 x 4096 x 4096 5.6
+// and 6.2 us, 1 x 14336 x 4096 16.2 and 15.4, 4 x 4096 x 28672 fp32 23.0 and
+// 21.1, 8 x 11008 x 4096 23.0 and 15.2, 16 x 4096 x 128256 95 and 83).
+constexpr int kW4Own = 2;
 struct W4Plan {
   int nt, rows, stages, kslice, slices, grid_x, grid_y;
   bool prepare;
