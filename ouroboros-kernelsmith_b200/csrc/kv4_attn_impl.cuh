@@ -34,7 +34,7 @@
 //     us instead of 135.)
 //     For float16 queries the probabilities take two products, p rounded and
 //     what that left: their rounding would show beside float16's own (32 x 8192
-//     tokens, g 32: 92 us instead of 84).
+//     tokens, g 32: 89 us instead of 82).
 //   * The running maximum and sum are fp32, per lane for its own tokens; the
 //     output is rescaled only when a row's maximum has moved by 2^4.
 //
@@ -1057,9 +1057,12 @@ static int attn_launch(const Kv4AttnArgs& a, const AttnPlan& p, cudaStream_t st)
                      : kv4_attn_kernel<D, GRP, NT, T, SPLIT, FINE>;
   allow_max_dynamic_smem(kern);
   launch_pdl(kern, dim3(p.blocks), dim3(32 * kAttnWarps), AttnShape<D, GRP, NT, T>::SMEM, st, a);
-  // a segment has about warps / segments parts
+  // A segment has about warps / segments parts; up to 16 a thread merges by
+  // itself (few against one block per row: 64 ragged sequences 54.3 and 59.2 us,
+  // 32 x 8192 tokens, 7 parts, 82.0 and 84.3; 8 x 65536, 28 parts, 122.7 and
+  // 117.3; 1 x 100000, 222 parts, 78 and 44).
   const unsigned rows = (unsigned)(a.Sq * a.G < 8 * NT ? a.Sq * a.G : 8 * NT);
-  if (p.segs >= 2 * sm_count())
+  if (p.segs * 16 >= p.warps)
     launch_pdl(kv4_attn_merge_few_kernel<D, NT>, dim3((unsigned)p.segs, (rows + 1024 / D - 1) / (1024 / D)),
                dim3(256), 0, st, a);
   else
