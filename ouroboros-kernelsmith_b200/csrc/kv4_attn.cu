@@ -4,12 +4,15 @@
 
 namespace b2k {
 
-// columns of the products, in eights: the fewest that hold the rows, up to
-// what the output's registers (NT D / 4 per thread) allow
+// Columns of the products, in eights: the fewest that hold the rows, two at
+// most, as the registers of four cost more than reading the cache again from
+// L2 (D 128: 16 x 8192 tokens, 32 rows a head, 107 us with two and 129 with
+// four, 8 x 8192, 256 rows, 374 and 422; one and two at 4 rows, 32 x 8192, 82
+// and 104).  With D 64 four hold up to 32 rows (16 x 8192, 20 rows, 68 us, with
+// two 77), but not more (35 rows of 16 ragged to 2500 18.1 and 14.9).
 static int attn_nt(int64_t rows, int64_t D) {
   if (rows <= 8) return 1;
-  if (rows <= 16 || D == 256) return 2;
-  return 4;
+  return D == 64 && rows > 16 && rows <= 32 ? 4 : 2;
 }
 
 static AttnPlan attn_plan(int64_t B, int64_t Sq, int64_t H, int64_t Hk, int64_t D) {

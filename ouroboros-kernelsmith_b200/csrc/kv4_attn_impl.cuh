@@ -1077,7 +1077,7 @@ static int attn_launch(const Kv4AttnArgs& a, const AttnPlan& p, cudaStream_t st)
 // per tile.
 template <int D, int GRP, int NT>
 static int attn_tokens(const Kv4AttnArgs& a, const AttnPlan& p, cudaStream_t st) {
-  if constexpr (D < 256 && NT * D <= 256) {
+  if constexpr (D < 256) {
     if (a.c.P % 32 == 0) return attn_launch<D, GRP, NT, 32, false>(a, p, st);
     return attn_launch<D, GRP, NT, 32, true>(a, p, st);
   } else {
@@ -1091,7 +1091,7 @@ static int attn_dispatch(const Kv4AttnArgs& a, const AttnPlan& p, cudaStream_t s
     case 1: return attn_tokens<D, GRP, 1>(a, p, st);
     case 2: return attn_tokens<D, GRP, 2>(a, p, st);
     default:
-      if constexpr (D < 256) return attn_tokens<D, GRP, 4>(a, p, st);
+      if constexpr (D == 64) return attn_tokens<D, GRP, 4>(a, p, st);
       return B2K_EUNSUPPORTED;
   }
 }
