@@ -5,20 +5,17 @@
 namespace b2k {
 
 // Columns of the products, in eights: the fewest that hold the rows, two at
-// most, as the registers of four cost more than reading the cache again from
-// L2 (D 128: 16 x 8192 tokens, 32 rows a head, 107 us with two and 129 with
-// four, 8 x 8192, 256 rows, 374 and 422; one and two at 4 rows, 32 x 8192, 82
-// and 104).  With D 64 four hold up to 32 rows (16 x 8192, 20 rows, 68 us, with
-// two 77), but not more (35 rows of 16 ragged to 2500 18.1 and 14.9).
-static int attn_nt(int64_t rows, int64_t D) {
-  if (rows <= 8) return 1;
-  return D == 64 && rows > 16 && rows <= 32 ? 4 : 2;
-}
+// most.  One and two at 4 rows a head: 32 x 8192 tokens 82 and 104 us.  Four
+// were slower: their registers cost more than reading the cache again from L2
+// (D 128, two and four: 16 x 8192 tokens with 32 rows 107 and 129 us, 8 x 8192
+// with 256 rows 374 and 422; D 64: 2 x 3000 with 32 rows 15.0 and 17.8, 16 x
+// 8192 with 20 rows 77 and 68, the one case that lost).
+static int attn_nt(int64_t rows) { return rows <= 8 ? 1 : 2; }
 
 static AttnPlan attn_plan(int64_t B, int64_t Sq, int64_t H, int64_t Hk, int64_t D) {
   AttnPlan p;
   const int64_t rows = Sq * (H / Hk);
-  p.nt = attn_nt(rows, D);
+  p.nt = attn_nt(rows);
   p.rt = (rows + 8 * p.nt - 1) / (8 * p.nt);
   p.blocks = sm_count() * attn_cps((int)D, p.nt);
   p.warps = p.blocks * kAttnWarps;

@@ -1072,9 +1072,9 @@ static int attn_launch(const Kv4AttnArgs& a, const AttnPlan& p, cudaStream_t st)
 }
 
 // Tiles of 32 tokens where registers hold their scores (NT T / 8 per thread
-// beside the output's NT D / 4), else of 16: 83 against 94 us at 16 sequences of
-// 16384 tokens, D 128.  Pages that are no multiple of 32 tokens take two copies
-// per tile.
+// beside the output's NT D / 4), up to D 128, else of 16: 83 against 94 us at 16
+// sequences of 16384 tokens, D 128.  Pages that are no multiple of 32 tokens
+// take two copies per tile.
 template <int D, int GRP, int NT>
 static int attn_tokens(const Kv4AttnArgs& a, const AttnPlan& p, cudaStream_t st) {
   if constexpr (D < 256) {
@@ -1087,13 +1087,7 @@ static int attn_tokens(const Kv4AttnArgs& a, const AttnPlan& p, cudaStream_t st)
 
 template <int D, int GRP>
 static int attn_dispatch(const Kv4AttnArgs& a, const AttnPlan& p, cudaStream_t st) {
-  switch (p.nt) {
-    case 1: return attn_tokens<D, GRP, 1>(a, p, st);
-    case 2: return attn_tokens<D, GRP, 2>(a, p, st);
-    default:
-      if constexpr (D == 64) return attn_tokens<D, GRP, 4>(a, p, st);
-      return B2K_EUNSUPPORTED;
-  }
+  return p.nt == 1 ? attn_tokens<D, GRP, 1>(a, p, st) : attn_tokens<D, GRP, 2>(a, p, st);
 }
 
 }  // namespace b2k
