@@ -482,8 +482,8 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // 2^(9 - floor(log2 top)); 1 for a row of zeros or one that is not finite
       const int ex = (int)(__float_as_uint(top) >> 23);
-      const float mag = top > 0.0f && ex < 255
-                            ? __uint_as_float((uint32_t)min(263 - ex, 254) << 23) : 1.0f;
+      const int me = top > 0.0f && ex < 255 ? min(263 - ex, 254) : 127;
+      const float mag = __uint_as_float((uint32_t)me << 23);
       const float f = a.scale < 0.0f ? -mag : mag;  // scores are multiplied by |scale|
       float part[NG];
 #pragma unroll
@@ -502,8 +502,10 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
                          as_u32(__halves2half2(h[1], h[5])), as_u32(__halves2half2(h[3], h[7]))};
         reinterpret_cast<uint4*>(qsm)[(nt * J + j) * 32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      // at least a number that leaves scale = 0 a factor of its own: 0 * -inf is NaN
-      const float cm = fmaxf(fabsf(a.scale) * kLog2e * (16777216.0f / mag), 1e-37f);
+      // |scale| log2(e) 2^24 / mag; the power of two alone may be past fp32's
+      // range (bfloat16 queries of 2^113 on).  At least a number that leaves
+      // scale = 0 a factor of its own: 0 * -inf is NaN
+      const float cm = fmaxf(scalbnf(fabsf(a.scale) * kLog2e, 24 + 127 - me), 1e-37f);
 #pragma unroll
       for (int p = 0; p < 2; ++p) {  // what this lane's columns 2c, 2c + 1 need
         const int src = (2 * c + p) * 4;

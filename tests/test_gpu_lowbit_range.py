@@ -1,0 +1,39 @@
+"""GPU tests of the low-precision serving ops at the ends of their ranges:
+queries and scales of magnitudes near the type's limits, arguments and values
+that are not numbers.
+
+Tolerances are those of test_gpu_lowbit.py: probabilities and values enter the
+products in float16 (2^-11 each), so |o - ref| <= 2^-9 max|v| + half an ulp of
+o; a product is off by 2^-16 of sum |x| s (w + z) and half an ulp of y.
+"""
+import pytest
+import torch
+
+import b200k
+from test_gpu_lowbit import HALF_ULP, attend64, fill, gen, make_tables, randn, values64
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(*values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("dim,group", [(64, 32), (128, 128), (256, 64)])
+@pytest.mark.parametrize("sq", [1, 5])
+@pytest.mark.parametrize("magnitude", [1e-35, 1e-20, 1e20, 1e33, 1e34, 1e35, 3e37])
+def test_attention_queries_over_the_whole_range_of_bfloat16(dim, group, sq, magnitude):
+    # the scale brings the scores back to ordinary numbers
+    g = gen(dim + sq)
+    cache, k, v = fill(g, 8, 2, 16, dim, group, torch.bfloat16)
+    table, lengths = make_tables(g, [100, 9], 16, 8)
+    q = randn(g, 2, sq, 8, dim).clamp(-4, 4).mul(magnitude).bfloat16()
+    kv = values64(cache, k, v)
+    scale = dim ** -0.5 / magnitude
+    for s in (scale, -scale):
+        ro, rl = attend64(q, kv, table, [100, 9], 16, scale=s)
+        o, lse = b200k.cache_attention(q, cache, table, lengths, scale=s, return_lse=True)
+        assert ((o.double() - ro).abs() <= 2.0 ** -9 * kv[1].abs().max() + 2.0 ** -8 * ro.abs()).all()
+        # fp32 sums of up to D products: 2^-18 of |q||k|, as the scale leaves it
+        mag = q.double().norm(dim=-1).max() * kv[0].norm(dim=-1).max() * abs(s)
+        assert ((lse.double() - rl).abs() <= 2.0 ** -18 * mag + 1e-5).all()
