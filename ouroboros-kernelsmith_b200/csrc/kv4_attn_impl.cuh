@@ -484,7 +484,9 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
       const int ex = (int)(__float_as_uint(top) >> 23);
       const int me = top > 0.0f && ex < 255 ? min(263 - ex, 254) : 127;
       const float mag = __uint_as_float((uint32_t)me << 23);
-      const float f = a.scale < 0.0f ? -mag : mag;  // scores are multiplied by |scale|
+      // scores are multiplied by |scale|; a scale of NaN goes in with the queries,
+      // so that what a row does not see stays at -inf
+      const float f = a.scale < 0.0f ? -mag : a.scale == a.scale ? mag : a.scale;
       float part[NG];
 #pragma unroll
       for (int g = 0; g < NG; ++g) part[g] = 0.0f;

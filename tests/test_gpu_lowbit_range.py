@@ -37,3 +37,17 @@ def test_attention_queries_over_the_whole_range_of_bfloat16(dim, group, sq, magn
         # fp32 sums of up to D products: 2^-18 of |q||k|, as the scale leaves it
         mag = q.double().norm(dim=-1).max() * kv[0].norm(dim=-1).max() * abs(s)
         assert ((lse.double() - rl).abs() <= 2.0 ** -18 * mag + 1e-5).all()
+
+
+@pytest.mark.parametrize("dim,group", [(64, 32), (128, 128)])
+def test_attention_scale_that_is_no_number(dim, group):
+    g = gen(dim)
+    cache, _, _ = fill(g, 4, 2, 16, dim, group, torch.bfloat16)
+    table, lengths = make_tables(g, [40, 0], 16, 4)
+    q = randn(g, 2, 1, 4, dim).bfloat16()
+    o, lse = b200k.cache_attention(q, cache, table, lengths, scale=float("nan"), return_lse=True)
+    assert o[0].isnan().all() and lse[0].isnan().all()
+    assert (o[1] == 0).all() and (lse[1] == -float("inf")).all()      # a row that sees nothing
+    # a scale of zero: every token counts alike
+    o, lse = b200k.cache_attention(q, cache, table, lengths, scale=0.0, return_lse=True)
+    assert o[0].isfinite().all() and (lse[0] - torch.log(torch.tensor(40.0))).abs().max() <= 1e-5
