@@ -959,7 +959,8 @@ __global__ void __launch_bounds__(D / 4 * kMergeSlices) kv4_attn_merge_kernel(
     for (int i = tid; i < n; i += THREADS) {
       const float2 p = *attn_ml(a, slot(base + i), ROWS * D);
       const float f = attn_weight(p.x, p.y, M);
-      weight[i] = f;
+      // -1: holds nothing; a part that weighs 0 is read, its output may be NaN
+      weight[i] = p.x == -INFINITY && p.y == 0.0f ? -1.0f : f;
       L = fmaf(p.y, f, L);
     }
     __syncthreads();
@@ -970,13 +971,13 @@ __global__ void __launch_bounds__(D / 4 * kMergeSlices) kv4_attn_merge_kernel(
       for (int j = 0; j < 8; ++j) {
         const int k = i + j * kMergeSlices;
         t[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (k < n && weight[k] != 0.0f)
+        if (k < n && weight[k] != -1.0f)
           t[j] = *reinterpret_cast<const float4*>(a.part + slot(base + k) * D + 4 * d4);
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int k = i + j * kMergeSlices;
-        const float f = k < n ? weight[k] : 0.0f;
+        const float f = k < n && weight[k] != -1.0f ? weight[k] : 0.0f;
         v.x = fmaf(t[j].x, f, v.x); v.y = fmaf(t[j].y, f, v.y);
         v.z = fmaf(t[j].z, f, v.z); v.w = fmaf(t[j].w, f, v.w);
       }

@@ -51,3 +51,28 @@ def test_attention_scale_that_is_no_number(dim, group):
     # a scale of zero: every token counts alike
     o, lse = b200k.cache_attention(q, cache, table, lengths, scale=0.0, return_lse=True)
     assert o[0].isfinite().all() and (lse[0] - torch.log(torch.tensor(40.0))).abs().max() <= 1e-5
+
+
+@pytest.mark.parametrize("dim,group", [(64, 32), (128, 128)])
+@pytest.mark.parametrize("batch,tokens,hk", [(1, 40000, 1), (3, 9000, 1), (64, 1500, 2)])
+def test_attention_a_nan_value_of_no_weight_reaches_its_dimensions(dim, group, batch, tokens, hk):
+    # scores so far apart that nearly every token, and every part that a long
+    # sequence is cut into, weighs 0 in fp32: 0 * NaN is NaN in each of them alike
+    g = gen(dim + batch)
+    page = 64
+    wide = -(-tokens // page)
+    cache, k, v = fill(g, batch * wide, hk, page, dim, group, torch.bfloat16)
+    table = torch.arange(batch * wide, dtype=torch.int32, device="cuda").view(batch, wide)
+    lengths = torch.full((batch,), tokens, dtype=torch.int32, device="cuda")
+    for step in (0, 1, 2):
+        at = torch.arange(batch, device="cuda") * wide * page + \
+            (torch.arange(batch, device="cuda") * 397 + step * tokens // 3) % tokens
+        part = v[at].clone()
+        part[:, 0, group - 1] = float("nan")
+        b200k.kv_cache_write(cache, k[at], part, at)
+        q = randn(g, batch, 1, 2 * hk, dim).bfloat16()
+        o, lse = b200k.cache_attention(q, cache, table, lengths, scale=20.0, return_lse=True)
+        nan = torch.zeros(o.shape, dtype=torch.bool, device="cuda")
+        nan[:, :, :2, :group] = True
+        assert torch.equal(o.isnan(), nan) and lse.isfinite().all()
+        b200k.kv_cache_write(cache, k[at], v[at], at)
