@@ -546,30 +546,37 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
       if (masked) {
         // What lies past the length is garbage, and a value some row does not
         // see must not reach it as 0 * NaN: such parameters become zero, and
-        // rows that do see a value that is not finite become NaN.
-        bool nan = false;
+        // rows that do see a value that is not finite become NaN in the
+        // dimensions of its group, as they do where every row sees it.
+        uint32_t odd = 0;  // the groups of lane's token
         const int tok = tok0 + lane;
         if (lane < T && tok > all_see) {
           uint32_t* p = reinterpret_cast<uint32_t*>(st + (lane >> 4) * MB + X::VP) + (lane & 15) * NG;
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
             const uint32_t w = p[g];
-            const bool odd = (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
-            if (tok >= end) p[g] = 0;
-            else if (odd) {
+            const bool bits = (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
+            if (tok >= end) {
               p[g] = 0;
-              nan = true;
+            } else if (bits) {
+              p[g] = 0;
+              odd |= 1u << g;
             }
           }
         }
-        uint32_t some = __ballot_sync(0xffffffffu, nan);
+        uint32_t some = __ballot_sync(0xffffffffu, odd != 0);
         for (; some; some &= some - 1) {
-          const int at = tok0 + __ffs(some) - 1;
+          const int from = __ffs(some) - 1;
+          const bool mine = __shfl_sync(0xffffffffu, odd, from) >> (r * (D / 8) / GRP) & 1u;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int p = 0; p < 2; ++p)
-              if (last_of(nt * 8 + 2 * c + p) >= at) l[nt][p] = __int_as_float(0x7fc00000);
+              if (mine && last_of(nt * 8 + 2 * c + p) >= tok0 + from) {
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+                  o[i][nt][p] = o[i][nt][2 + p] = __int_as_float(0x7fc00000);
+              }
         }
         __syncwarp();
       }

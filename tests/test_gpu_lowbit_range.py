@@ -76,3 +76,38 @@ def test_attention_a_nan_value_of_no_weight_reaches_its_dimensions(dim, group, b
         nan[:, :, :2, :group] = True
         assert torch.equal(o.isnan(), nan) and lse.isfinite().all()
         b200k.kv_cache_write(cache, k[at], v[at], at)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,group,page", [(64, 32, 16), (64, 64, 32), (128, 32, 64), (128, 64, 16),
+                                            (128, 128, 64), (256, 32, 16), (256, 128, 32)])
+def test_attention_a_partly_nan_value_reaches_its_own_dimensions_only(dtype, dim, group, page):
+    # one group of one token's value is NaN: in every row that sees the token the
+    # dimensions of that group are NaN, the others and the log-sum numbers,
+    # whichever other rows and tokens it is computed with
+    g = gen(dim + group + page)
+    tokens, sq = 71, 9
+    pages = -(-96 // page)
+    cache, k, v = fill(g, pages, 2, page, dim, group, dtype)
+    kv = values64(cache, k, v)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    q = randn(g, 1, sq, 8, dim).to(dtype)
+    for at in (3, 62, 64, 66, 68, 70):             # the last four seen by some queries only
+        for first in range(0, dim, group):
+            part = v[at:at + 1].clone()
+            part[:, 1, first] = float("nan")       # of the second head alone
+            b200k.kv_cache_write(cache, k[at:at + 1], part, torch.tensor([at], device="cuda"))
+            ro, rl = attend64(q, kv, table, [tokens], page)
+            o, lse = b200k.cache_attention(q, cache, table, i32(tokens), return_lse=True)
+            nan = torch.zeros(1, sq, 8, dim, dtype=torch.bool, device="cuda")
+            nan[:, max(0, at - (tokens - sq)):, 4:, first:first + group] = True
+            assert torch.equal(o.isnan(), nan)
+            err = (o.double() - ro).abs()
+            assert (err <= 2.0 ** -9 * kv[1].abs().max() + HALF_ULP[dtype] * ro.abs())[~nan].all()
+            mag = q.double().norm(dim=-1).max() * kv[0].norm(dim=-1).max() * dim ** -0.5
+            assert ((lse.double() - rl).abs() <= 2.0 ** -18 * mag + 1e-5).all()
+            # each query by itself gives the same answer
+            for i in (0, 4, 8):
+                one = b200k.cache_attention(q[:, i:i + 1], cache, table, i32(tokens - sq + 1 + i))
+                assert torch.equal(one.isnan(), nan[:, i:i + 1])
+        b200k.kv_cache_write(cache, k[at:at + 1], v[at:at + 1], torch.tensor([at], device="cuda"))
