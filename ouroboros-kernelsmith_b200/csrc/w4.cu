@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const T* w, int64_t ld
 // in fp32: x' is x in float16 after a power of two xs that brings the largest
 // of the group's columns to [2^14, 2^15), so 16-bit x is exact unless it is
 // 2^-25 of its group's maximum; float32 x takes two columns, x' = hi + 2^-11 lo
-// (22 bits).  8-bit x is exact as it is and xs is its scale.
+// (22 bits).  8-bit x is exact (x' = 128 x) and xs goes by its scale.
 //
 // Blocks are persistent, one per SM, and hold all of x (their slice of K) in
 // shared memory, prepared once.  A block takes an equal share of the row tiles
@@ -262,7 +262,10 @@ __device__ __forceinline__ void w4_stage_eight(const W4Args& a, int64_t row, int
   float f = 1.0f, xs;
   if (a.xs) {
     const int64_t g = a.xgroup ? k / a.xgroup : 0;
-    xs = live && k < a.w.K ? a.xs[row * a.ldxs + g] * 16384.0f : 0.0f;
+    // half of the units' 2^14 in the values, where it is exact (448 * 128 fits
+    // float16), so that the scales of the largest fp32 rows stay finite
+    f = 128.0f;
+    xs = live && k < a.w.K ? a.xs[row * a.ldxs + g] * 128.0f : 0.0f;
     // a group of 8-bit values that are not finite, or of such a scale, is NaN
     bool odd = false;
 #pragma unroll

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import b200k
-from test_gpu_lowbit import HALF_ULP, attend64, fill, gen, make_tables, randn, values64
+from test_gpu_lowbit import HALF_ULP, attend64, fill, gen, make_tables, make_weight, randn, values64
 
 pytestmark = pytest.mark.gpu
 
@@ -111,3 +111,23 @@ def test_attention_a_partly_nan_value_reaches_its_own_dimensions_only(dtype, dim
                 one = b200k.cache_attention(q[:, i:i + 1], cache, table, i32(tokens - sq + 1 + i))
                 assert torch.equal(one.isnan(), nan[:, i:i + 1])
         b200k.kv_cache_write(cache, k[at:at + 1], v[at:at + 1], torch.tensor([at], device="cuda"))
+
+
+@pytest.mark.parametrize("xt", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("factor", [1e-37, 1e-30, 1e30, 1e34, 1e35, 1.5e36])
+@pytest.mark.parametrize("m,per", [(1, None), (5, 64)])
+def test_product_scales_of_8_bit_rows_over_the_whole_range(xt, factor, m, per):
+    # up to what float32 rows are quantised with, 3.4e38 / 127; eight columns that
+    # count, weights of about 1e-2: y is a number
+    g = gen(m)
+    n, k, group = 48, 320, 64
+    w, q, s, zp = make_weight(g, n, k, group, True)
+    x = randn(g, m, k) * 4
+    x[:, 8:] = 0
+    x = (x.round() if xt == torch.int8 else x).to(xt)
+    xs = (torch.rand((m, k // per if per else 1), generator=g, device="cuda") + 0.5) * factor
+    y = b200k.w4_matmul(x, w, x_scale=xs, out_dtype=torch.float32)
+    xd = x.double() * (xs.double().repeat_interleave(per, 1) if per else xs.double())
+    ref = xd @ (s.double() * (q.double() - zp)).T
+    a = xd.abs() @ (s.double() * (q.double() + zp)).T
+    assert ((y.double() - ref).abs() <= 2.0 ** -16 * a + 2.0 ** -24 * ref.abs() + 2.0 ** -146).all()
