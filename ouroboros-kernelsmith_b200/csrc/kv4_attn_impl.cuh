@@ -51,6 +51,7 @@
 #pragma once
 
 #include "kv4_attn_plan.cuh"
+#include "kv4_span.cuh"
 #include "rowio.cuh"
 #include "rowpipe.cuh"
 
@@ -226,6 +227,38 @@ __device__ __forceinline__ void attn_step(const Kv4AttnArgs& a, AttnWalk& k) {
     k.n = 0;
     ++k.entry;
   }
+}
+
+// A run in which a wait ran out, from the part at hand on: its parts are NaN,
+// and accounted for like others, as the merges go by what the workspace says.
+// Not inline: the kernel's registers are for the way that is taken.
+template <int D, int NT, int T>
+__device__ __noinline__ void attn_give_up(const Kv4AttnArgs& a, AttnWalk use, int run, int64_t u1,
+                                          int64_t each, int64_t more) {
+  constexpr int ROWS = attn_rows(NT);
+  const int lane = threadIdx.x & 31;
+  const float nan = __int_as_float(0x7fc00000);
+  do {
+    const bool whole = use.t == 0 && use.t1 == use.n;
+    if (use.t == 0 && lane == 0) {
+      const int64_t last = u1 - use.left - use.pos + use.n + use.lead - 1;  // unit
+      const int64_t to = last < more * (each + 1) ? last / (each + 1) : more + (last - more * (each + 1)) / each;
+      a.spans[(int64_t)use.entry * a.c.Hk + use.head] = make_int2(run, whole ? run : (int)to);
+    }
+    const int b = a.dRT.div(use.entry), row0 = (use.entry - b * a.RT) * ROWS;
+    const int64_t slot = 2 * (int64_t)run + (use.t == 0 ? 1 : 0);
+    for (int row = 0; row < ROWS && row0 + row < (int)(a.Sq * a.G); ++row) {
+      if (!whole) {
+        if (lane == 0) *attn_ml(a, slot * ROWS + row, ROWS * D) = make_float2(-INFINITY, nan);
+        continue;
+      }
+      const int i = a.dG.div(row0 + row), hq = use.head * a.G + (row0 + row - i * a.G);
+      uint16_t* dst = static_cast<uint16_t*>(a.o) + (((int64_t)b * a.Sq + i) * a.H + hq) * D;
+      for (int d = lane; d < D; d += 32) dst[d] = 0x7fff;  // NaN in both types
+      if (a.lse && lane == 0) a.lse[((int64_t)b * a.H + hq) * a.Sq + i] = nan;
+    }
+    attn_step(a, use);
+  } while (attn_next<D, NT, T>(a, use));
 }
 
 template <int D, int GRP, int NT, int T, bool SPLIT, bool FINE>
@@ -530,7 +563,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
 
     for (int t = t0; t < t1; ++t) {
       const int s = use_stage;
-      if (!mbar_wait(&full[warp][s], use_phase)) {
+      if (!mbar_wait_warp(&full[warp][s], use_phase)) {
         timeout = true;
         break;
       }
@@ -861,9 +894,17 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
       }
     attn_step(a, use);
   }
-  if (timeout) {  // nothing may land after the block has gone
-    for (; used < issued; ++used) mbar_wait(&full[warp][used % S], (used / S) & 1);
-    if (lane == 0) atomicAdd(&b2k_tu_timeouts, 1u);
+  if (timeout) {
+    // nothing may land after the block has gone
+    for (; used < issued; ++used) mbar_wait_warp(&full[warp][used % S], (used / S) & 1);
+    if (lane == 0) {
+      atomicAdd(&b2k_tu_timeouts, 1u);
+      first_segment[0] = use.entry;
+      first_segment[1] = use.head;
+    }
+    my_first = use.t == 0;
+    my_last = use.t1 == use.n;
+    attn_give_up<D, NT, T>(a, use, (int)run, u1, each, more);
   }
   if (!one_segment) return;
 
@@ -878,7 +919,7 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
       const int row = nt * 8 + 2 * c + p;
       if (r == 0) {
         mrg[warp][row][0] = m[nt][p];
-        mrg[warp][row][1] = l[nt][p];
+        mrg[warp][row][1] = timeout ? __int_as_float(0x7fc00000) : l[nt][p];
       }
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
@@ -946,9 +987,10 @@ __global__ void __launch_bounds__(D / 4 * kMergeSlices) kv4_attn_merge_kernel(
   const int64_t seg = blockIdx.x;
   const int row = blockIdx.y, tid = threadIdx.x, slice = tid / (D / 4), d4 = tid - slice * (D / 4);
   const int2 span = a.spans[seg];
-  if (span.x == span.y) return;
+  const int parts = attn_parts(span.x, span.y, a.warps);
+  if (parts == 0) return;
   const int entry = a.dHk.div((int)seg), b = a.dRT.div(entry), head = (int)seg - entry * a.c.Hk;
-  const int rr = (entry - b * a.RT) * ROWS + row, parts = span.y - span.x + 1;
+  const int rr = (entry - b * a.RT) * ROWS + row;
   if (rr >= (int)(a.Sq * a.G)) return;
   auto slot = [&](int i) { return (2 * (int64_t)(span.x + i) + (i == 0 ? 1 : 0)) * ROWS + row; };
   float M = -INFINITY;
@@ -1020,9 +1062,10 @@ __global__ void __launch_bounds__(256) kv4_attn_merge_few_kernel(const __grid_co
   const int seg = blockIdx.x, row = blockIdx.y * (1024 / D) + threadIdx.x / (D / 4);
   const int d = threadIdx.x % (D / 4) * 4;
   const int2 span = a.spans[seg];
-  if (span.x == span.y) return;
+  const int parts = attn_parts(span.x, span.y, a.warps);
+  if (parts == 0) return;
   const int entry = a.dHk.div(seg), b = a.dRT.div(entry), head = seg - entry * a.c.Hk;
-  const int rr = (entry - b * a.RT) * ROWS + row, parts = span.y - span.x + 1;
+  const int rr = (entry - b * a.RT) * ROWS + row;
   if (row >= ROWS || rr >= (int)(a.Sq * a.G)) return;
   auto slot = [&](int i) { return (2 * (int64_t)(span.x + i) + (i == 0 ? 1 : 0)) * ROWS + row; };
   float M = -INFINITY, L = 0.0f;

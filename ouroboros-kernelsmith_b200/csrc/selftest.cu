@@ -1,6 +1,7 @@
 // Self-test of the bounded-wait path used by every pipelined kernel: one
 // block waits on an mbarrier that nothing ever completes, with a short limit,
-// and must give up, count the timeout and return (the context stays usable).
+// each thread for itself and then as a warp, and must give up both times, count
+// one timeout and return (the context stays usable).
 // No copy is issued, so nothing is in flight when the block exits.
 #include "tma.cuh"
 
@@ -15,7 +16,9 @@ __global__ void selftest_wait_kernel(unsigned long long limit_ns, int* status) {
     fence_barrier_init();
   }
   __syncthreads();
-  const bool done = mbar_wait(&bar, 0u, limit_ns);
+  bool done = mbar_wait(&bar, 0u, limit_ns);
+  __syncthreads();
+  done |= mbar_wait_warp(&bar, 0u, limit_ns);  // the block is one warp
   __syncthreads();
   if (threadIdx.x == 0) {
     if (!done) atomicAdd(&b2k_tu_timeouts, 1u);

@@ -122,6 +122,18 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
   }
 }
 
+// mbar_wait by all lanes of a warp, with one answer for all of them: whichever
+// it is, the lanes are together for the warp's collective instructions.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity,
+                                               unsigned long long limit_ns = kTimeoutNs) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const unsigned long long t0 = globaltimer();
+  for (uint32_t i = 1;; ++i) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((i & 255u) == 0 && __any_sync(0xffffffffu, globaltimer() - t0 > limit_ns)) return false;
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Thread-block cluster primitives (distributed shared memory between the
 // CTAs of one cluster on this GPU; no multicast).
