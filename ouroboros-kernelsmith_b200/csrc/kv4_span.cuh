@@ -2,11 +2,7 @@
 // C++, so that a test can compile it by itself.
 #pragma once
 
-#ifdef __CUDACC__
-#define B2K_HOST_DEVICE __host__ __device__ __forceinline__
-#else
-#define B2K_HOST_DEVICE inline
-#endif
+#include "host_device.cuh"
 
 namespace b2k {
 

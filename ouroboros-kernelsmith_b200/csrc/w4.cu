@@ -12,6 +12,7 @@
 #include <cuda_fp8.h>
 #include <limits.h>
 
+#include "ring.cuh"
 #include "rowio.cuh"
 #include "rowpipe.cuh"
 
@@ -404,9 +405,10 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * kW4War
   };
   const Walk begin = {before, 0, 0, body};
   Walk get = begin;
-  int get_stage = 0, use_stage = 0;
-  uint32_t use_phase = 0, issued = 0, used = 0;
-  bool dead = false;  // a wait ran out
+  int get_stage = 0;
+  uint32_t issued = 0;
+  RingUse taken;
+  auto arrived = [&](int stage, uint32_t phase) { return mbar_wait_warp(&full[warp][stage], phase); };
   int64_t get_at = 0;  // block of the item's (first) tile in the layout
   int get_left = 0;    // blocks of it to come
   bool getting = false;
@@ -466,10 +468,7 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * kW4War
         bulk_g2s(xsm + o, xw + kb0 * 256 * C + o, min(xb - o, 32768u), &xbar);
       bulk_g2s(gsm, xw + KT * 256 * (f32 ? 2 * a.rows : a.rows) + kb0 * GS * 64 * NT, gb, &xbar);
     }
-    if (!mbar_wait(&xbar, 0)) {
-      dead = true;
-      if (lane == 0) atomicAdd(&b2k_tu_timeouts, 1u);
-    }
+    taken.dead = !mbar_wait_warp(&xbar, 0);  // then nothing is taken from the ring
   } else {
     for (int i = tid; i < kn * GS * 8 * NT; i += blockDim.x) gsm[i] = f2(0.0f, 0.0f);
     __syncthreads();
@@ -516,17 +515,8 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * kW4War
   Walk use = begin;
   while (u0 < u1 && next_item(use)) {
     for (int k = use.k; k < use.end; k += SBK) {
-      const int stage = use_stage;
-      if (!dead && !mbar_wait(&full[warp][stage], use_phase)) {
-        // go on to the block's barrier; the results are lost
-        dead = true;
-        if (lane == 0) atomicAdd(&b2k_tu_timeouts, 1u);
-      }
-      ++used;
-      if (++use_stage == S) {
-        use_stage = 0;
-        use_phase ^= 1;
-      }
+      const int stage = taken.take(S, arrived);
+      if (stage < 0) break;
       const unsigned char* st = ring + stage * STAGE;
 #pragma unroll
       for (int i = 0; i < SBK; ++i) {
@@ -586,8 +576,9 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * kW4War
         }
       }
       __syncwarp();
-      if (getting && !dead) issue();
+      if (getting) issue();
     }
+    if (taken.dead) break;
     if (use.at == INT_MAX) break;  // the head stays in y
     const bool ends = use.end == kn;
     const int64_t item = i0 + use.item;
@@ -619,9 +610,22 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * kW4War
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[nt][e] = 0.0f;
   }
-  if (dead)  // nothing may land where the parts go
-    for (used -= used > 0; used < issued; ++used)
-      mbar_wait(&full[warp][used % S], (used / S) & 1);
+  if (taken.dead) {  // a wait ran out: nothing may land where the parts go, or later
+    taken.drain(issued, S, arrived);
+    if (a.xw) mbar_wait_warp(&xbar, 0);
+    if (lane == 0) atomicAdd(&b2k_tu_timeouts, 1u);
+    // the item at hand and those to come are NaN
+    while (u0 < u1 && use.at != INT_MAX) {
+      if (use.end != kn) {
+        tail_item = use.item;
+      } else {
+        for (int i = lane; i < rows * 16; i += 32)
+          store(i >> 4, (i0 + use.item) * 16 + (i & 15), __int_as_float(0x7fc00000));
+      }
+      ++use.item;
+      if (!next_item(use)) break;
+    }
+  }
 
   // ---- items that span warps: their parts, in the warps' drained rings ----------
   if (kn == 0) {  // no columns at all
@@ -638,8 +642,9 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * kW4War
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int at = (nt * 8 + 2 * c + (e & 1)) * 16 + (e >> 1 ? row_b : row_a);
-        mine[at] = y[nt][e];  // zeros where there is no head
-        if (has_tail) mine[PER + at] = tail[nt][e];
+        // zeros where there is no head
+        mine[at] = taken.dead ? __int_as_float(0x7fc00000) : y[nt][e];
+        if (has_tail) mine[PER + at] = taken.dead ? __int_as_float(0x7fc00000) : tail[nt][e];
       }
   __syncthreads();
   // this warp's tail, and the heads of the next warps whose runs lie in that item
