@@ -362,7 +362,8 @@ int b2k_kv4_attention(const void* q, int64_t qb, int64_t qs, int64_t qh, void* o
  * Laid out as tiles [ceil(N/16), ceil(K/128), 16 rows, 64 bytes], 32-bit word
  * 4c + j of a row holding columns 32j + 8c .. + 7 of its 128 (the first column
  * in the low bits), and scales / zeros [ceil(N/16), ceil(K/128), 128/group,
- * 16]; what lies past N or K is 0. */
+ * 16]; what lies past N or K is 0.  All three start at 16 bytes, and so does
+ * the product's workspace. */
 
 /* Lays out integers q (N,K) and scales / zeros (N, ceil(K/group)). */
 int b2k_w4_pack(const uint8_t* q, int64_t ldq, const void* scales, const void* zeros,

@@ -763,6 +763,13 @@ static int w4_check(const char* what, int64_t N, int64_t K, int group, int stype
   return B2K_OK;
 }
 
+// the product copies all three in bulk
+static int w4_check_aligned(const char* what, const void* tiles, const void* scales, const void* zeros) {
+  B2K_REQUIRE(aligned16(tiles) && aligned16(scales) && aligned16(zeros),
+              "%s: the tiles, their scales and zeros must be 16-byte aligned", what);
+  return B2K_OK;
+}
+
 static unsigned w4_blocks(int64_t items) {
   const int64_t b = (items + 255) / 256;
   return (unsigned)(b < 65536 ? (b < 1 ? 1 : b) : 65536);
@@ -779,6 +786,7 @@ extern "C" int b2k_w4_pack(const uint8_t* q, int64_t ldq, const void* scales, co
   if (N == 0 || K == 0) return B2K_OK;
   B2K_REQUIRE(q && scales && tiles && tile_scales && (!zeros == !tile_zeros),
               "b2k_w4_pack: null operand");
+  if (int st = w4_check_aligned("b2k_w4_pack", tiles, tile_scales, tile_zeros)) return st;
   W4PackArgs a = {q, ldq, scales, zeros, lds, static_cast<unsigned char*>(tiles), tile_scales,
                   tile_zeros, N, K, group};
   const int64_t nk = ((N + 15) / 16) * ((K + 127) / 128);
@@ -794,6 +802,7 @@ extern "C" int b2k_w4_quantize(const void* w, int64_t ldw, int64_t N, int64_t K,
   if (int st = w4_check("b2k_w4_quantize", N, K, group, stype)) return st;
   if (N == 0 || K == 0) return B2K_OK;
   B2K_REQUIRE(w && tiles && tile_scales, "b2k_w4_quantize: null operand");
+  if (int st = w4_check_aligned("b2k_w4_quantize", tiles, tile_scales, tile_zeros)) return st;
   const int64_t items = ((N + 15) / 16) * ((K + 127) / 128) * (128 / group) * 16;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   B2K_DISPATCH_FLOAT(dtype, {
@@ -833,6 +842,8 @@ extern "C" int b2k_w4_matmul(const void* x, int64_t ldx, int xtype, const float*
   B2K_REQUIRE(M >= 0 && M <= 0x7fffffffLL, "b2k_w4_matmul: bad number of rows %lld", (long long)M);
   if (M == 0 || N == 0) return B2K_OK;
   B2K_REQUIRE(y && (K == 0 || (x && tiles && tile_scales)), "b2k_w4_matmul: null operand");
+  if (K > 0)
+    if (int st = w4_check_aligned("b2k_w4_matmul", tiles, tile_scales, tile_zeros)) return st;
   B2K_REQUIRE(M <= 1 || (ldx >= K && ldy >= N), "b2k_w4_matmul: row stride smaller than the row");
   W4Args a = {};
   a.w = W4{static_cast<const unsigned char*>(tiles), tile_scales, tile_zeros, N, K, group};
