@@ -382,7 +382,8 @@ def w4_matmul(x, weight: W4Weight, *, x_scale=None, out_dtype: torch.dtype | Non
     [..., 1] or [..., ceil(k / g)] for groups of g = 32, 64 or 128 columns, a
     multiple of the weight's group (what rmsnorm_quant returns).  out_dtype
     defaults to x's dtype (bfloat16 for 8-bit x).  Meant for few rows: the
-    weights are read once for every 32 of them.  A row that holds an infinity
+    weights are read once for every 32 of them (8 of float32, whose products keep
+    float32's precision).  A row that holds an infinity
     or a NaN comes out NaN."""
     if not isinstance(weight, W4Weight):
         raise TypeError(f"b200k: expected a W4Weight, got {type(weight).__name__}")

@@ -134,14 +134,22 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const T* w, int64_t ld
 //
 // in fp32: x' is x in float16 after a power of two xs that brings the largest
 // of the group's columns to [2^14, 2^15), so 16-bit x is exact unless it is
-// 2^-25 of its group's maximum; float32 x takes two columns, x' = hi + 2^-11 lo
-// (22 bits).  8-bit x is exact (x' = 128 x) and xs goes by its scale.
+// 2^-25 of its group's maximum; float32 x takes three columns, x' = hi + 2^-11
+// mid + 2^-22 lo.  Of these hi and mid are multiples of 16, up to 2^15 and 2^14:
+// their products with the integers, and the sums of 128, are multiples of 16 below
+// 2^26, so nothing of them is lost beside a column that is much larger than the
+// others.  (The matrix instruction drops what lies 24 bits below its largest term:
+// two columns of 11 leading bits each were off by 2^-17 of the result in such
+// rows, and took 21.1 us instead of 29.8 at 4 x 4096 x 28672, 45.7 instead of 88
+// with 16 rows.)  A row takes four columns, the last empty.  8-bit x is exact (x'
+// = 128 x) and xs goes by its scale.
 //
 // Blocks are persistent, one per SM, and hold all of x (their slice of K) in
 // shared memory, prepared once.  A block takes an equal share of the row tiles
 // and its warps equal runs of their blocks of 128 columns, whatever tile these
 // lie in; a tile that spans warps is added up at the end.  Every warp has its
 // own ring of bulk copies, which runs ahead across tiles.
+constexpr int kW4F32 = 4;  // columns of a row of float32
 constexpr int kW4Stages = 4, kW4Smem = 226 << 10;  // stages at most; of an SM's memory
 
 struct W4Args {
@@ -292,18 +300,21 @@ __device__ __forceinline__ void w4_stage_eight(const W4Args& a, int64_t row, int
       xs = __uint_as_float((uint32_t)(268 - fb) << 23);
     }
   }
-  for (int part = 0; part < (f32 ? 2 : 1); ++part) {
-    const int col = f32 ? 2 * m + part : m;
+  for (int part = 0; part < (f32 ? 3 : 1); ++part) {
+    const int col = f32 ? kW4F32 * m + part : m;
     __half h[8], h16[8];
     float sum = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float t = part == 0 ? v[e] * f : v[e];
+      float t = part == 0 ? v[e] * f : v[e];
+      const float all = t;
+      // float32: multiples of 16, first of x' and then of 2^11 times the rest
+      if (f32 && part < 2) t = rintf(t * 0.0625f) * 16.0f;
       h[e] = __float2half_rn(t);
       const float back = __half2float(h[e]);
       sum += back;
       h16[e] = __float2half_rn(back * 0.0625f);
-      v[e] = (t - back) * 2048.0f;
+      v[e] = (all - back) * 2048.0f;
     }
 #pragma unroll
     for (int o = 1; o < G / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -312,8 +323,11 @@ __device__ __forceinline__ void w4_stage_eight(const W4Args& a, int64_t row, int
           make_uint4(h2_bits(h[0], h[4]), h2_bits(h[2], h[6]), h2_bits(h16[1], h16[5]),
                      h2_bits(h16[3], h16[7]));
       // the sum in units of the products, 2^-24
-      if (v8 % (G / 8) == 0)
-        go[(int64_t)(v8 / (G / 8)) * pitch + col] = f2(sum * 5.9604644775390625e-8f, xs);
+      if (v8 % (G / 8) == 0) {
+        float2* to = go + (int64_t)(v8 / (G / 8)) * pitch + col;
+        to[0] = f2(sum * 5.9604644775390625e-8f, xs);
+        if (f32 && part == 2) to[1] = f2(0.0f, 0.0f);  // the row's fourth column
+      }
     }
   }
 }
@@ -328,7 +342,7 @@ __global__ void __launch_bounds__(256) w4_x_kernel(const __grid_constant__ W4Arg
   // and what came before this grid may have written them.
   griddep_launch_dependents();
   const int64_t KT = a.w.ktiles(), per_row = KT * 16;
-  const int per = a.xtype == B2K_F32 ? 2 : 1, cols = a.rows * per;
+  const int per = a.xtype == B2K_F32 ? kW4F32 : 1, cols = a.rows * per;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t y = blockIdx.y, m0 = y * a.rows;
   const int rows = (int)min((int64_t)a.rows, a.M - m0);
@@ -343,10 +357,10 @@ __global__ void __launch_bounds__(256) w4_x_kernel(const __grid_constant__ W4Arg
       go[(int64_t)(v8 / (16 / GS)) * 8 * nt + col] = f2(0.0f, 0.0f);
 }
 
-// GS = groups per 128 columns, 8 NT = columns (rows of x; two each for
-// float32), BF: scales and zeros are bfloat16
-template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * kW4Warps, 1) w4_kernel(
-    const __grid_constant__ W4Args a) {
+// GS = groups per 128 columns, 8 NT = columns (rows of x; four each for
+// float32, F32), BF: scales and zeros are bfloat16
+template <int NT, int GS, bool BF, bool F32>
+__global__ void __launch_bounds__(32 * kW4Warps, 1) w4_kernel(const __grid_constant__ W4Args a) {
   constexpr int G = 128 / GS, STAGE = w4_stage(GS);
   constexpr int SBK = kW4Blocks, W = kW4Warps;
   const int S = a.stages;
@@ -358,11 +372,12 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * kW4War
   const int kn = (int)min((int64_t)a.kslice, KT - kb0);  // blocks of this slice
   const int64_t m0 = (int64_t)blockIdx.y * a.rows;
   const int rows = (int)min((int64_t)a.rows, a.M - m0);
-  const bool f32 = a.xtype == B2K_F32, zeros = a.w.zeros != nullptr;
-  const int C = f32 ? 2 * rows : rows;
+  const bool zeros = a.w.zeros != nullptr;
+  constexpr int per = F32 ? kW4F32 : 1;
+  const int C = per * rows;
   unsigned char* ring = smem + warp * (S * STAGE);
   unsigned char* xsm = smem + W * (S * STAGE);
-  float2* gsm = reinterpret_cast<float2*>(xsm + w4_x_bytes(a.kslice, f32 ? 2 * a.rows : a.rows));
+  float2* gsm = reinterpret_cast<float2*>(xsm + w4_x_bytes(a.kslice, per * a.rows));
   // 16 zero bytes, what lanes past the last column read
   const uint32_t nothing = (uint32_t)(reinterpret_cast<unsigned char*>(gsm) - smem) +
                            (uint32_t)w4_g_bytes(a.kslice, GS, NT);
@@ -460,13 +475,13 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * kW4War
     }
     __syncthreads();
     if (tid == 0) {
-      const unsigned char* xw = a.xw + (int64_t)blockIdx.y * w4_image_bytes(KT, f32 ? 2 * a.rows : a.rows, GS, NT);
+      const unsigned char* xw = a.xw + (int64_t)blockIdx.y * w4_image_bytes(KT, per * a.rows, GS, NT);
       const uint32_t xb = kn * 256 * C, gb = kn * GS * 64 * NT;
       fence_proxy_async();
       mbar_arrive_expect_tx(&xbar, xb + gb);
       for (uint32_t o = 0; o < xb; o += 32768)
         bulk_g2s(xsm + o, xw + kb0 * 256 * C + o, min(xb - o, 32768u), &xbar);
-      bulk_g2s(gsm, xw + KT * 256 * (f32 ? 2 * a.rows : a.rows) + kb0 * GS * 64 * NT, gb, &xbar);
+      bulk_g2s(gsm, xw + KT * 256 * (per * a.rows) + kb0 * GS * 64 * NT, gb, &xbar);
     }
     taken.dead = !mbar_wait_warp(&xbar, 0);  // then nothing is taken from the ring
   } else {
@@ -494,7 +509,7 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * kW4War
     else if (a.ytype == B2K_F16) static_cast<__half*>(a.y)[at] = from_f<__half>(v);
     else static_cast<__nv_bfloat16*>(a.y)[at] = from_f<__nv_bfloat16>(v);
   };
-  constexpr float kLow = 0.00048828125f;  // 2^-11, the weight of float32's second column
+  constexpr float kLow = 0.00048828125f;  // 2^-11, from a column of float32 to the next
 
   float y[NT][4];
 #pragma unroll
@@ -506,7 +521,7 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * kW4War
   uint32_t xat[NT], xstep[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const bool in = nt * 8 + r < C;
+    const bool in = nt * 8 + r < C && !(F32 && (r & 3) == 3);
     xat[nt] = in ? (uint32_t)(xsm - smem) + (nt * 8 + r) * 64 + c * 16 : nothing;
     xstep[nt] = in ? C * 64 : 0;
   }
@@ -597,8 +612,9 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * kW4War
             const int64_t n = item * 16 + (h ? row_b : row_a);
             const float v0 = y[nt][2 * h], v1 = y[nt][2 * h + 1];
             const int col = nt * 8 + 2 * c;
-            if (f32) {
-              if (col < C) store(col >> 1, n, fmaf(v1, kLow, v0));
+            if (F32) {
+              const float v2 = __shfl_down_sync(0xffffffffu, v0, 1);  // columns 2c + 2
+              if (!(c & 1) && col < C) store(col / kW4F32, n, fmaf(v2, kLow * kLow, fmaf(v1, kLow, v0)));
             } else {
               if (col < C) store(col, n, v0);
               if (col + 1 < C) store(col + 1, n, v1);
@@ -655,15 +671,17 @@ template <int NT, int GS, bool BF> __global__ void __launch_bounds__(32 * kW4War
   for (int w = 1; w < W; ++w) last += w > warp && run_at(w) < past;
   for (int i = lane; i < rows * 16; i += 32) {
     const int m = i >> 4, n16 = i & 15;
-    const int c0 = (f32 ? 2 * m : m) * 16 + n16, c1 = f32 ? c0 + 16 : c0;
-    float v = mine[PER + c0], low = mine[PER + c1];
+    const int c0 = per * m * 16 + n16;
     const float* from = reinterpret_cast<const float*>(smem);
+    float v = 0.0f;
+    for (int part = F32 ? 2 : 0; part >= 0; --part) {
+      const int at = c0 + part * 16;
+      float t = mine[PER + at];
 #pragma unroll 4
-    for (int w = warp + 1; w <= last; ++w) {
-      v += from[w * (S * STAGE / 4) + c0];
-      low += from[w * (S * STAGE / 4) + c1];
+      for (int w = warp + 1; w <= last; ++w) t += from[w * (S * STAGE / 4) + at];
+      v = fmaf(v, kLow, t);
     }
-    store(m, (i0 + tail_item) * 16 + n16, f32 ? fmaf(low, kLow, v) : v);
+    store(m, (i0 + tail_item) * 16 + n16, v);
   }
 }
 
@@ -686,8 +704,7 @@ template <typename T> __global__ void __launch_bounds__(256) w4_sum_kernel(const
 // x does not fit beside that.  x is prepared once by a kernel of its own where
 // every block's own preparation would take it more than kW4Own eights of
 // columns per thread (own preparation against the kernel: 1 x 4096 x 4096 5.6
-// and 6.2 us, 1 x 14336 x 4096 16.2 and 15.4, 4 x 4096 x 28672 fp32 23.0 and
-// 21.1, 8 x 11008 x 4096 23.0 and 15.2, 16 x 4096 x 128256 95 and 83).
+// and 6.2 us, 1 x 14336 x 4096 16.2 and 15.4, 8 x 11008 x 4096 23.0 and 15.2, 16 x 4096 x 128256 95 and 83).
 constexpr int kW4Own = 2;
 struct W4Plan {
   int nt, rows, stages, kslice, slices, grid_x, grid_y;
@@ -697,7 +714,7 @@ struct W4Plan {
 
 static W4Plan w4_plan(int64_t M, int64_t N, int64_t K, int group, bool f32) {
   W4Plan p;
-  const int per = f32 ? 2 : 1, gs = 128 / group;
+  const int per = f32 ? kW4F32 : 1, gs = 128 / group;
   const int64_t cols = M * per, KT = (K + 127) / 128, tiles = (N + 15) / 16;
   p.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
   p.rows = (int)(M < 8 * p.nt / per ? M : 8 * p.nt / per);
@@ -732,7 +749,7 @@ template <int NT, int GS, bool BF> static void w4_launch(const W4Args& a, const 
     const int64_t eights = (int64_t)p.rows * a.w.ktiles() * 16;
     launch_pdl(w4_x_kernel<GS>, dim3((unsigned)((eights + 255) / 256), p.grid_y), dim3(256), 0, st, a, NT);
   }
-  auto kern = w4_kernel<NT, GS, BF>;
+  auto kern = a.xtype == B2K_F32 ? w4_kernel<NT, GS, BF, true> : w4_kernel<NT, GS, BF, false>;
   allow_max_dynamic_smem(kern);
   launch_pdl(kern, dim3(p.grid_x, p.grid_y, p.slices), dim3(32 * kW4Warps), (size_t)p.smem, st, a);
 }

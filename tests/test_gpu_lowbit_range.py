@@ -131,3 +131,28 @@ def test_product_scales_of_8_bit_rows_over_the_whole_range(xt, factor, m, per):
     ref = xd @ (s.double() * (q.double() - zp)).T
     a = xd.abs() @ (s.double() * (q.double() + zp)).T
     assert ((y.double() - ref).abs() <= 2.0 ** -16 * a + 2.0 ** -24 * ref.abs() + 2.0 ** -146).all()
+
+
+@pytest.mark.parametrize("m,n,k,group,zeros", [(1, 604, 1145, 128, True), (2, 604, 1145, 128, True),
+                                               (3, 100, 1000, 32, True), (5, 333, 4096, 128, False),
+                                               (8, 64, 640, 64, True), (19, 48, 2000, 64, False),
+                                               (2, 96, 28672, 128, True)])
+@pytest.mark.parametrize("loud", [1.0, 20.0, 100.0])
+def test_product_of_float32_rows_keeps_float32(m, n, k, group, zeros, loud):
+    # Some columns are `loud` times the others, as hidden states have them.  x in
+    # parts of whole units makes a group's sums exact; what is left are three fp32
+    # roundings a group and one for adding it up, each 2^-24 at most and 0.3 of
+    # 2^-23 in the mean square, of partial sums that are at most the result's size
+    # in the mean square: over G groups sqrt(G) 2^-24.7 of it, and the roundings
+    # of a group's own share, which is sqrt(1/G) of it.
+    g = gen(m + k)
+    w, q, s, zp = make_weight(g, n, k, group, zeros)
+    x = randn(g, m, k)
+    x[:, torch.rand(k, generator=g, device="cuda") < 0.01] *= loud
+    y = b200k.w4_matmul(x, w).double()
+    ref = x.double() @ (s.double() * (q.double() - zp)).T
+    groups = -(-k // group)
+    bound = 1.2 * 2.0 ** -24.7 * (groups + 3) ** 0.5
+    assert (y - ref).norm() <= bound * ref.norm(), float((y - ref).norm() / ref.norm())
+    one = b200k.w4_matmul(x[m - 1:], w).double()     # the last row by itself
+    assert (one - ref[m - 1:]).norm() <= 1.2 * bound * ref[m - 1:].norm()
