@@ -32,9 +32,10 @@
 //     The running maximum is that of p s, so that these products use float16's
 //     range whatever the values' magnitude.  (8 x 65536 tokens, D 128, g 128: 118
 //     us instead of 135.)
-//     For float16 queries the probabilities take two products, p rounded and
-//     what that left: their rounding would show beside float16's own (32 x 8192
-//     tokens, g 32: 89 us instead of 82).
+//     For float16 queries the probabilities take two products, p (or p s)
+//     rounded and what that left: their rounding would show beside float16's own
+//     (errors 1.4 to 1.6 times those of fp32 products; 32 x 8192 tokens, g 32: 90
+//     us instead of 83).
 //   * The running maximum and sum are fp32, per lane for its own tokens; the
 //     output is rescaled only when a row's maximum has moved by 2^4.
 //
@@ -779,9 +780,13 @@ kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
         }
         if constexpr (X::FOLD) {  // -8 for every dimension, in the units of the two rows
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt) {
             mma16816(eight[nt], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, pf[u][nt][0],
                      pf[u][nt][1]);
+            if constexpr (FINE)
+              mma16816(eight[nt], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, pr[u][nt][0],
+                       pr[u][nt][1]);
+          }
         }
         const __half2 s0 = as_h2(__byte_perm(par[0], par[1], 0x5410));
         const __half2 o0 = as_h2(__byte_perm(par[0], par[1], 0x7632));
@@ -1107,9 +1112,8 @@ __global__ void __launch_bounds__(256) kv4_attn_merge_few_kernel(const __grid_co
 
 template <int D, int GRP, int NT, int T, bool SPLIT>
 static int attn_launch(const Kv4AttnArgs& a, const AttnPlan& p, cudaStream_t st) {
-  constexpr bool FINE = GRP < D;  // for float16
   auto kern = a.bf16 ? kv4_attn_kernel<D, GRP, NT, T, SPLIT, false>
-                     : kv4_attn_kernel<D, GRP, NT, T, SPLIT, FINE>;
+                     : kv4_attn_kernel<D, GRP, NT, T, SPLIT, true>;
   allow_max_dynamic_smem(kern);
   launch_pdl(kern, dim3(p.blocks), dim3(32 * kAttnWarps), AttnShape<D, GRP, NT, T>::SMEM, st, a);
   // A segment has about warps / segments parts; up to 16 a thread merges by

@@ -14,7 +14,8 @@ evenly in their logarithm its mean square is (u/2)^2 / 3 * 0.541, that is
 
 with r operand roundings a term: one (the value lo + s n) for float16 queries,
 whose probabilities are held in two parts; two (value, probability) for
-bfloat16; one (p s) for a single group per head, whose integers are exact.
+bfloat16; with a single group per head, whose integers are exact, one (p s) for
+bfloat16 and none for float16 (the last test; the others allow one).
 fp32 scores add relative errors of about 1e-6.  Checked with 10 % above; one
 more rounding of a float16 call's operands would be 22 % above.
 """
@@ -108,7 +109,7 @@ def attend64(q, kv, table, lens, page, scale):
     return o, noise, lse
 
 
-def attend_case(seed, dtype, lens, sq, heads, hk, dim, group, page, offset=0.0):
+def attend_case(seed, dtype, lens, sq, heads, hk, dim, group, page, offset=0.0, rounded=None):
     """Every element within 2^-9 of its own share sum_j p_j |v_j|, and all of
     them within the mean square above."""
     g = gen(seed)
@@ -132,7 +133,8 @@ def attend_case(seed, dtype, lens, sq, heads, hk, dim, group, page, offset=0.0):
     err = (o.double() - ro).permute(0, 2, 1, 3)[~empty]
     noise, ro = (t.permute(0, 2, 1, 3)[~empty] for t in (noise, ro))
     half = HALF_ULP[dtype]
-    rounded = 2 if dtype == torch.bfloat16 and group < dim else 1
+    if rounded is None:
+        rounded = 2 if dtype == torch.bfloat16 and group < dim else 1
     want = 0.4246 * (rounded * 2.0 ** -22 * noise.mean() + half ** 2 * (ro * ro).mean()).sqrt()
     got = (err * err).mean().sqrt()
     assert got <= 1.1 * want, (float(got), float(want))
@@ -175,3 +177,12 @@ def test_attention_of_over_1024_parts(dtype, dim, group, sq, heads):
     # one segment, cut into a run of four tiles and less for every warp: more
     # parts than the merge holds at a time
     attend_case(5, dtype, [150001], sq, heads, 1, dim, group, 64)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens,sq,heads,hk", [([700, 33, 0, 1500], 1, 8, 2), ([900, 40], 5, 14, 2),
+                                              ([16384], 1, 8, 2), ([60000, 777], 1, 7, 1),
+                                              ([20001], 3, 8, 1)])
+def test_attention_of_float16_over_one_group_rounds_only_its_output(dim, lens, sq, heads, hk):
+    # integers are exact and probabilities held in two parts: r = 0
+    attend_case(dim + sq, torch.float16, lens, sq, heads, hk, dim, dim, 64, rounded=0)
