@@ -744,6 +744,9 @@ static W4Plan w4_plan(int64_t M, int64_t N, int64_t K, int group, bool f32) {
   return p;
 }
 
+// rows of x in one launch: 65535 blocks of 32 columns
+static int64_t w4_most_rows(bool f32) { return (int64_t)65535 * 32 / (f32 ? kW4F32 : 1); }
+
 template <int NT, int GS, bool BF> static void w4_launch(const W4Args& a, const W4Plan& p, cudaStream_t st) {
   if (p.prepare) {
     const int64_t eights = (int64_t)p.rows * a.w.ktiles() * 16;
@@ -839,7 +842,15 @@ extern "C" int64_t b2k_w4_matmul_workspace(int64_t M, int64_t N, int64_t K, int 
   if (M < 0 || N < 0 || K < 0 || M > 0x7fffffffLL || (group != 32 && group != 64 && group != 128))
     return -1;
   if (M == 0 || N == 0) return 0;
-  return w4_plan(M, N, K, group, xtype == B2K_F32).bytes;
+  // the chunks that the product takes its rows in use it one after another
+  const int64_t most = w4_most_rows(xtype == B2K_F32);
+  int64_t bytes = 0;
+  for (int64_t m : {M < most ? M : most, M % most})
+    if (m > 0) {
+      const int64_t b = w4_plan(m, N, K, group, xtype == B2K_F32).bytes;
+      bytes = b > bytes ? b : bytes;
+    }
+  return bytes;
 }
 
 extern "C" int b2k_w4_matmul(const void* x, int64_t ldx, int xtype, const float* xs, int64_t ldxs,
@@ -862,13 +873,25 @@ extern "C" int b2k_w4_matmul(const void* x, int64_t ldx, int xtype, const float*
   if (K > 0)
     if (int st = w4_check_aligned("b2k_w4_matmul", tiles, tile_scales, tile_zeros)) return st;
   B2K_REQUIRE(M <= 1 || (ldx >= K && ldy >= N), "b2k_w4_matmul: row stride smaller than the row");
+  const int64_t most = w4_most_rows(xtype == B2K_F32);
+  if (M > most) {
+    const char* xb = static_cast<const char*>(x);
+    char* yb = static_cast<char*>(y);
+    for (int64_t m = 0; m < M; m += most)
+      if (int st = b2k_w4_matmul(xb + m * ldx * dtype_size(xtype), ldx, xtype, xs ? xs + m * ldxs : xs,
+                                 ldxs, xgroup, tiles, tile_scales, tile_zeros, stype, group,
+                                 M - m < most ? M - m : most, N, K, yb + m * ldy * dtype_size(ytype), ldy,
+                                 ytype, workspace, workspace_bytes, stream))
+        return st;
+    return B2K_OK;
+  }
   W4Args a = {};
   a.w = W4{static_cast<const unsigned char*>(tiles), tile_scales, tile_zeros, N, K, group};
   a.x = x; a.ldx = ldx; a.xs = xs; a.ldxs = ldxs; a.xgroup = xgroup;
   a.y = y; a.ldy = ldy; a.M = M;
   a.xtype = xtype; a.ytype = ytype; a.stype = stype;
   const W4Plan p = w4_plan(M, N, K, group, xtype == B2K_F32);
-  B2K_REQUIRE(p.grid_y <= 65535 && p.slices <= 65535, "b2k_w4_matmul: shape too large");
+  B2K_REQUIRE(p.slices <= 65535, "b2k_w4_matmul: shape too large");
   B2K_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes && aligned16(workspace)),
               "b2k_w4_matmul: the workspace needs %lld bytes, got %lld", (long long)p.bytes,
               (long long)workspace_bytes);

@@ -156,3 +156,18 @@ def test_product_of_float32_rows_keeps_float32(m, n, k, group, zeros, loud):
     assert (y - ref).norm() <= bound * ref.norm(), float((y - ref).norm() / ref.norm())
     one = b200k.w4_matmul(x[m - 1:], w).double()     # the last row by itself
     assert (one - ref[m - 1:]).norm() <= 1.2 * bound * ref[m - 1:].norm()
+
+
+@pytest.mark.parametrize("xt,m", [(torch.float32, 65535 * 8 + 5), (torch.float32, 65535 * 8),
+                                  (torch.bfloat16, 65535 * 32 + 33), (torch.int8, 65535 * 32 + 1)])
+def test_product_of_more_rows_than_one_launch_takes(xt, m):
+    g = gen(9)
+    w, q, s, zp = make_weight(g, 16, 40, 32, True)
+    x = randn(g, m, 40)
+    xs = torch.rand((m, 1), generator=g, device="cuda") + 0.5 if xt == torch.int8 else None
+    x = (x * 30).round().clamp(-127, 127).to(xt) if xs is not None else x.to(xt)
+    y = b200k.w4_matmul(x, w, x_scale=xs, out_dtype=torch.float32).double()
+    xd = x.double() if xs is None else x.double() * xs.double()
+    wd = s.double() * (q.double() - zp)
+    a = xd.abs() @ (s.double() * (q.double() + zp)).T
+    assert y.shape == (m, 16) and ((y - xd @ wd.T).abs() <= 2.0 ** -16 * a).all()
