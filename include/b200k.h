@@ -347,8 +347,10 @@ int64_t b2k_kv4_attention_workspace(int64_t B, int64_t Sq, int64_t H, int64_t Hk
  * included.  Head h reads cache head h / (H/Hk).  With causal != 0 query i
  * sees tokens up to lens - Sq + i.  o (B, Sq, H, D) contiguous in dtype;
  * lse (B, H, Sq) fp32 or NULL.  A row that sees nothing is zeros (lse -inf);
- * a length beyond width*P, or a page outside the pool among the tokens read,
- * gives NaN for the rows concerned.  The workspace is scratch of
+ * a length beyond width*P gives NaN for its sequence, a page outside the pool
+ * among the tokens read NaN for the rows that see it and for rows computed with
+ * them (up to 16 of a cache head), a value that is not finite NaN in the
+ * dimensions of its group for the rows that see it.  The workspace is scratch of
  * b2k_kv4_attention_workspace bytes (16-byte aligned), needs no
  * initialisation, and is free again when the call's GPU work has run. */
 int b2k_kv4_attention(const void* q, int64_t qb, int64_t qs, int64_t qh, void* o, float* lse,
@@ -379,9 +381,13 @@ int b2k_w4_quantize(const void* w, int64_t ldw, int64_t N, int64_t K, int dtype,
 /* y (M,N) = x (M,K) W^T with fp32 sums.  x is a floating dtype, or B2K_I8 /
  * B2K_E4M3 with fp32 scales xs (M, xgroup ? ceil(K/xgroup) : 1), xgroup a
  * multiple of the weight's group up to 128.  y is a floating dtype.  A row of
- * x that holds an infinity or a NaN gives NaN.  Few rows of x are held on chip
- * whole; where they do not fit, K is split and the workspace holds partial
- * sums (b2k_w4_matmul_workspace bytes, 0 mostly; needs no initialisation). */
+ * x that holds an infinity or a NaN gives NaN.  Rows of x are held on chip;
+ * where every block would take long to bring them into the form of the products
+ * (more than 1024 eights of columns) that is done once, in the workspace, and
+ * where they do not fit, K is split and the workspace holds partial sums too:
+ * b2k_w4_matmul_workspace bytes, 0 for a few short rows; needs no
+ * initialisation, and is free again when the call's GPU work has run.  A
+ * workspace larger than that is fine. */
 int64_t b2k_w4_matmul_workspace(int64_t M, int64_t N, int64_t K, int group, int xtype);
 int b2k_w4_matmul(const void* x, int64_t ldx, int xtype, const float* xs, int64_t ldxs,
                   int xgroup, const void* tiles, const void* tile_scales,

@@ -12,6 +12,10 @@ synchronisation, TypeError / ValueError before a launch, B200KError when one
 fails.  Indices that only the device knows (slots, pages, lengths) are checked
 by the kernels: a slot outside the pool is not written, and what cannot be
 read becomes NaN in the rows that asked for it.
+
+These ops serve: their results carry no gradient, also where an input requires
+one.  What is trained through a product with frozen 4-bit weights needs that
+product's gradient from elsewhere.
 """
 from __future__ import annotations
 
@@ -246,8 +250,10 @@ def cache_attention(q, cache: KVCache4, page_table, lengths, *, scale: float | N
     lengths - Sq + i; a row that sees none is zeros (log-sum -inf).  scale
     defaults to D ** -0.5.  Returns o [B, Sq, H, D] in q's dtype, and with
     return_lse also the log of the sum of exponentials, fp32 [B, H, Sq].  A
-    length beyond the table, or a page outside the pool among the tokens read,
-    gives NaN for that sequence."""
+    length beyond the table gives NaN for its sequence; a page outside the pool
+    among the tokens read for the rows that see it, and for rows computed with
+    them; a value that is not finite in the dimensions of its group, for the rows
+    that see its token.  No gradient."""
     _check_cache(cache)
     dev = _cuda(q, cache.data, page_table, lengths)
     dt = _dt16(q.dtype, "q")
@@ -384,7 +390,7 @@ def w4_matmul(x, weight: W4Weight, *, x_scale=None, out_dtype: torch.dtype | Non
     defaults to x's dtype (bfloat16 for 8-bit x).  Meant for few rows: the
     weights are read once for every 32 of them (8 of float32, whose products keep
     float32's precision).  A row that holds an infinity
-    or a NaN comes out NaN."""
+    or a NaN comes out NaN.  No gradient, neither to x nor to the weights."""
     if not isinstance(weight, W4Weight):
         raise TypeError(f"b200k: expected a W4Weight, got {type(weight).__name__}")
     dev = _cuda(x, weight.tiles, x_scale)

@@ -30,7 +30,7 @@
 //     same for every dimension, is summed apart and settled every four tiles: left
 //     to the end, the sums would exceed the output by the square root of the tokens.
 //     The running maximum is that of p s, so that these products use float16's
-//     range whatever the values' magnitude.  (8 x 65536 tokens, D 128, g 128: 118
+//     range whatever the values' magnitude.  (8 x 65536 tokens, D 128, g 128: 119
 //     us instead of 135.)
 //     For float16 queries the probabilities take two products, p (or p s)
 //     rounded and what that left: their rounding would show beside float16's own

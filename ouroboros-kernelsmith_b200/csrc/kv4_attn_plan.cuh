@@ -30,7 +30,10 @@ struct Kv4AttnArgs {
 
 // rows of a row tile
 __host__ __device__ constexpr int attn_rows(int NT) { return 8 * NT; }
-// resident blocks per SM: registers (NT D / 4 for the output) and shared memory
+// resident blocks per SM: registers (NT D / 4 for the output) and shared memory.
+// Three leave 168 registers, which D 128 with groups of 32, D 64 with 16 rows and D
+// 256 exceed by 4 to 10 (spilled); two leave 255, which D 256 with 16 rows exceeds
+// by 9 to 22.  One block more spilled far more and was slower.
 __host__ __device__ constexpr int attn_cps(int D, int NT) { return NT * D >= 256 && NT > 1 ? 2 : 3; }
 
 struct AttnPlan {
