@@ -389,7 +389,8 @@ def w4_matmul(x, weight: W4Weight, *, x_scale=None, out_dtype: torch.dtype | Non
     multiple of the weight's group (what rmsnorm_quant returns).  out_dtype
     defaults to x's dtype (bfloat16 for 8-bit x).  Meant for few rows: the
     weights are read once for every 32 of them (8 of float32, whose products keep
-    float32's precision).  A row that holds an infinity
+    float32's precision; those of 16-bit and 8-bit x are good to about 2^-17 of the
+    result beside columns 20 to 100 times the others).  A row that holds an infinity
     or a NaN comes out NaN.  No gradient, neither to x nor to the weights."""
     if not isinstance(weight, W4Weight):
         raise TypeError(f"b200k: expected a W4Weight, got {type(weight).__name__}")
